@@ -207,6 +207,9 @@ __device__ __forceinline__ void gat_fwd_group_online(const GatParams &p, uint32_
 template <int G, bool MAP, class C>
 __device__ __forceinline__ void gat_bwd_col_group(const GatParams &p, uint32_t q, uint32_t h, uint32_t f, bool on, uint32_t ls, float lun,
                                                   const float4 &hn, float &dan, float4 &acc) {
+  // (the roundings are spelled out -- which products fuse into sums is otherwise the compiler's choice per instantiation -- so that
+  //  the MAP and the dense form give the same bits)
+#pragma clang fp contract(off)
   uint32_t s_[G], m_[G];
   float us[G], mx[G], dn[G], t[G], w[G];
   float4 v[G];
@@ -236,8 +239,9 @@ __device__ __forceinline__ void gat_bwd_col_group(const GatParams &p, uint32_t q
     // alpha_ij dN_i . hn_j alone, and the subtracted row maximum no longer cancels: -t_i reaches the maximum edge (kept or dropped
     // by the edge mask) the way torch_scatter's max hands its gradient to the arg-max (shaDow/layers.py:572-578)
     const float tt = (dn[j] > 1e-10f) ? alpha * t[j] : (ev == mx[j] ? t[j] : 0.f);
-    dan += alpha * dal - tt;
-    acc.x += alpha * v[j].x; acc.y += alpha * v[j].y; acc.z += alpha * v[j].z; acc.w += alpha * v[j].w;
+    dan += __builtin_fmaf(alpha, dal, -tt);
+    acc.x = __builtin_fmaf(alpha, v[j].x, acc.x); acc.y = __builtin_fmaf(alpha, v[j].y, acc.y);
+    acc.z = __builtin_fmaf(alpha, v[j].z, acc.z); acc.w = __builtin_fmaf(alpha, v[j].w, acc.w);
   }
 }
 // group sizes tried before the single-edge tail: bit masks of {8, 4, 2} per kernel (round 3, on the round-3 kernels; same box, products
@@ -398,7 +402,8 @@ __device__ __forceinline__ void gat_col_bwd_body(const GatParams &p) {
     if (on) {
       const float dun = dan * dlrelu02(unr);
       float4 dzv;
-      acc.x += dun * a1.x; acc.y += dun * a1.y; acc.z += dun * a1.z; acc.w += dun * a1.w;
+      acc.x = __builtin_fmaf(dun, a1.x, acc.x); acc.y = __builtin_fmaf(dun, a1.y, acc.y);
+      acc.z = __builtin_fmaf(dun, a1.z, acc.z); acc.w = __builtin_fmaf(dun, a1.w, acc.w);
       if (p.z_neigh) {
         dzv = make_float4(acc.x * g_act_bwd(p.act, z.x, hn.x), acc.y * g_act_bwd(p.act, z.y, hn.y),
                           acc.z * g_act_bwd(p.act, z.z, hn.z), acc.w * g_act_bwd(p.act, z.w, hn.w));
@@ -408,7 +413,8 @@ __device__ __forceinline__ void gat_col_bwd_body(const GatParams &p) {
       }
       gst4(p.dz_neigh + r * F + f, dzv);
       rmax = shadow::amax4(dzv);
-      g1.x += dun * hn.x; g1.y += dun * hn.y; g1.z += dun * hn.z; g1.w += dun * hn.w;
+      g1.x = __builtin_fmaf(dun, hn.x, g1.x); g1.y = __builtin_fmaf(dun, hn.y, g1.y);
+      g1.z = __builtin_fmaf(dun, hn.z, g1.z); g1.w = __builtin_fmaf(dun, hn.w, g1.w);
     }
     if (p.row_amax) {                    // joined with the maximum of dz_self's row (accumulate mode: the caller's; otherwise zero rows)
       rmax = shadow::group_max<LPR>(rmax);

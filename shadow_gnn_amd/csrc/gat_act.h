@@ -38,7 +38,10 @@ __device__ __forceinline__ float g_act_bwd_h(int act, float h) {
 __device__ __forceinline__ float4 act4(int act, float4 z) {
   return make_float4(g_act_fwd(act, z.x), g_act_fwd(act, z.y), g_act_fwd(act, z.z), g_act_fwd(act, z.w));
 }
-__device__ __forceinline__ float gat_dot4(float4 a, float4 b) { return a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w; }
+// (fused products by name: which sums fuse is otherwise the compiler's choice per kernel)
+__device__ __forceinline__ float gat_dot4(float4 a, float4 b) {
+  return __builtin_fmaf(a.w, b.w, __builtin_fmaf(a.z, b.z, __builtin_fmaf(a.y, b.y, a.x * b.x)));
+}
 
 // sum over the ls lanes of a head slice (ls power of two, wave-uniform): DPP butterflies (actnorm_common.h)
 __device__ __forceinline__ float slice_sum(float v, uint32_t ls) {
