@@ -215,10 +215,8 @@ class MinibatchShallowExtractor:
         # > 0: every batch carries up to that many nested levels of a row-sparse backward pass instead (GAT stacks on deep
         # subgraphs: tail.build_backward_levels)
         self.backward_levels = 0
-        # (priority -1 = high: when the deferred sampler call meets the GEMMs of the step, its workgroups take the CU slots
-        #  as they free up instead of queueing behind the GEMM's grid; SHADOW_PREFETCH_PRIORITY=0 for a normal stream)
-        prio = int(os.environ.get("SHADOW_PREFETCH_PRIORITY", "-1"))
-        self._side = torch.cuda.Stream(device=self.device, priority=prio) if self.prefetch else None
+        # (a stream of the default priority: work on streams of different priorities has hung on these GPUs)
+        self._side = torch.cuda.Stream(device=self.device) if self.prefetch else None
         # prefetch launched when the consumer reaches ops.fire_deferred (see ops.DEFER_POINT: once the GNN layers of the forward
         # pass are enqueued) instead of at once: it then runs in the nearly idle read-out / loss stretch of the step instead of
         # on its HBM-bound head (round-3 A/B); SHADOW_DEFER_PREFETCH=0 restores the immediate launch
