@@ -924,6 +924,53 @@ int sl_gat_bwd_map(const uint32_t *d_indptr, const uint32_t *d_indices, const ui
                    const float *d_dnagg_rows, const float *d_t_rows, const uint32_t *d_dn_map, float *d_work, float *d_dz_self,
                    float *d_dz_neigh, float *d_datt, int accumulate_dz_self, float *d_row_amax, void *stream);
 
+/* ---------------------------------------------------------------- node-wise MLP operators (ABI 26)
+ * Element types of the operands.  Rows have a pitch (ld*, in elements, at least the row's width); no alignment is required --
+ * rows of whole 16-byte words take the fastest path.  Statistics, sums and scores are fp32 whatever the type.  Nothing is allocated,
+ * cleared with a memset node or kept between calls: every entry may be captured into a graph. */
+#define SL_F32 0
+#define SL_BF16 1
+#define SL_F16 2
+/* y = (x - mean) (var + eps)^-1/2 * scale + offset over rows of F elements (1 <= F <= 16384; biased variance, two-pass).  scale /
+ * offset [F] of type w_dtype (SL_F32 or dtype), each may be NULL (1 / 0).  d_stats (may be NULL): [n, 2] mean and (var + eps)^-1/2 of
+ * every row, which the backward pass reads.  (The normalisation of shaDow/layers.py:329-338 without its activation.) */
+int sl_layer_norm_fwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, const void *d_scale, const void *d_offset, uint32_t n,
+                      uint32_t F, float eps, void *d_y, int64_t ldy, float *d_stats, void *stream);
+/* dx, dscale [F], doffset [F] (each may be NULL); d_partial: sl_layer_norm_partial_floats(n, F) floats, needed for dscale / doffset.
+ * n == 0 writes zeros there. */
+size_t sl_layer_norm_partial_floats(uint32_t n, uint32_t F);
+int sl_layer_norm_bwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const void *d_scale,
+                      const float *d_stats, uint32_t n, uint32_t F, void *d_dx, int64_t lddx, void *d_dscale, void *d_doffset,
+                      float *d_partial, void *stream);
+/* y[r, c] = (d_res ? res[r, c] : 0) + (keep(r, c) ? x[r, c] / (1 - p) : 0), 0 <= p < 1, with the mask rule of the fused epilogues
+ * (csrc/actnorm_common.h): the same (p, seed) keeps the same elements.  d_seed (may be NULL): the seed is read from device memory when
+ * the kernel runs, so that a replayed graph can be given a new one.  A dropped element is 0 whatever x holds.  The backward pass is
+ * the same call on dy without d_res. */
+int sl_dropout(int dtype, const void *d_x, int64_t ldx, const void *d_res, int64_t ldr, uint64_t n, uint32_t F, float p, uint64_t seed,
+               const int64_t *d_seed, void *d_y, int64_t ldy, void *stream);
+/* y = act(x W^T + bias) + res: x [M, K], W [N, K], res and y [M, N] in bf16 or fp16, bias [N] in that type or fp32; bias / res may be
+ * NULL.  act: 0 identity, 1 relu, 2 elu, 3 tanh, 4 leakyrelu(0.2), 5 gelu, 6 silu.  d_z (may be NULL): the pre-activations in fp16,
+ * pitch ldz a multiple of 8 and 16-byte aligned, for the backward pass. */
+int sl_linear16_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, int bias_f32, const void *d_res,
+                    int64_t ldr, uint32_t M, uint32_t N, uint32_t K, int act, void *d_y, int64_t ldy, void *d_z, int64_t ldz, void *stream);
+/* dx [M, K], dW [N, K], db [N] (each may be NULL; db only together with dW) from dy and d_z (act != 0; pitch: N rounded up to 8).
+ * The rows of dz^T x are cut into slices whose products are added in slice order (no atomics). */
+size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K);
+int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy, const void *d_z,
+                    int64_t ldz, uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, void *d_db,
+                    int db_f32, void *d_scratch, void *stream);
+/* Rows of C logits with a label each (int32 or int64; < 0: no label, log probability 0; >= C: NaN): log probability of the label,
+ * entropy of the softmax, and the k <= min(C, 64) largest logits' log probabilities and indices (value descending, lowest index first,
+ * NaN on top).  A logit of -inf has probability 0; a row without a finite logit answers -inf, entropy 0 and has gradient 0; +inf or
+ * NaN anywhere makes the row NaN.  d_stat [n, 2]: the row's maximum and log2-sum below it, read by the backward pass. */
+size_t sl_label_logprobs_scratch_bytes(int dtype, uint32_t n, uint32_t C, uint32_t k);
+int sl_label_logprobs_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_label, int label_i64, uint32_t n, uint32_t C, uint32_t k,
+                          float *d_logprob, float *d_entropy, float *d_stat, float *d_top_lp, int64_t *d_top_idx, void *d_scratch, void *stream);
+/* dx from the gradients of the log probabilities, entropies and alternatives' log probabilities (each may be NULL). */
+int sl_label_logprobs_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_label, int label_i64, uint32_t n, uint32_t C, uint32_t k,
+                          const float *d_stat, const float *d_entropy, const int64_t *d_top_idx, const float *d_dlogprob,
+                          const float *d_dentropy, const float *d_dtop, void *d_dx, int64_t lddx, void *stream);
+
 /* Development aid: per-subgraph result words of the last sg_sample call,
  * 16 uint32 per subgraph: {nodes, edges, flags, stream slots, frontier nodes,
  * frontier reads, -, -, 8 x phase cycle stamps (only when the library was

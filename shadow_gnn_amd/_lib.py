@@ -264,13 +264,26 @@ SIGNATURES = {
     "sl_act_norm_bwd_map": (C.c_int, [C.c_int, C.POINTER(_P), C.POINTER(C.c_int64), C.POINTER(_P), C.POINTER(C.c_int), _P, _P,
                                       C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, _P, C.c_int64, _P,
                                       C.POINTER(_P), C.POINTER(C.c_int64), _P, _P, _P, _P, C.c_float, C.c_uint64, _P, C.c_int64, _P, _P]),
+    "sl_layer_norm_fwd": (C.c_int, [C.c_int, C.c_int, _P, C.c_int64, _P, _P, C.c_uint32, C.c_uint32, C.c_float, _P, C.c_int64, _P, _P]),
+    "sl_layer_norm_partial_floats": (C.c_size_t, [C.c_uint32, C.c_uint32]),
+    "sl_layer_norm_bwd": (C.c_int, [C.c_int, C.c_int, _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_uint32, C.c_uint32, _P, C.c_int64, _P, _P, _P, _P]),
+    "sl_dropout": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, C.c_uint64, C.c_uint32, C.c_float, C.c_uint64, _P, _P, C.c_int64, _P]),
+    "sl_linear16_fwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+                                  _P, C.c_int64, _P, C.c_int64, _P]),
+    "sl_linear16_bwd_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "sl_linear16_bwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+                                  _P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, _P]),
+    "sl_label_logprobs_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "sl_label_logprobs_fwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P, _P, _P]),
+    "sl_label_logprobs_bwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P, _P, _P,
+                                        C.c_int64, _P]),
 }
 
 _lib = None
 
 
 MAX_BATCHES_PER_CALL = 16      # SG_MAX_BATCHES_PER_CALL of include/shadow_hip.h
-ABI_VERSION = 25      # sg_abi_version() of the library these signatures describe
+ABI_VERSION = 26      # sg_abi_version() of the library these signatures describe
 
 
 def load():
