@@ -2,11 +2,11 @@
 // in its epilogue, and its gradients:
 //     z = x W^T + b,   y = act(z) + res,   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum_rows dz
 //
-// One tile kernel serves x W^T and dz W (the weight transposed once per call, it is small), a second one dz^T x.
-// 128 x 128 output tiles, 64 steps of the contraction per stage, two stages in LDS (64 KB: two workgroups share a CU and cover each
-// other's barriers), four wavefronts of 64 x 64 on 32x32x16 products.  A tile's rows are 128 bytes of the operand; the 16-byte words of
-// row r sit at word ^ ((r >> 1) & 7), so that the 16 lanes that read together hit 16 different bank groups.
-// The products are formed as W x^T: a lane then holds four neighbouring output COLUMNS of a row.
+// Three kernels for x W^T and dz W (the weight transposed once per call, it is small): 256 x 256 tiles for large products, 128 x 128
+// for the others, 32 x 32 with the contraction cut over wavefronts where there are few tiles; one for dz^T x.
+// Tiles are staged in LDS 64 steps of the contraction at a time -- 128 bytes of every row: with half lines (32 steps) every line
+// crossed to the CU twice, 338 instead of 314 us at 32768 x 1024 x 4096 -- and multiplied on 32x32x16 products formed as W x^T: a lane then
+// holds four neighbouring output COLUMNS of a row.
 // Operands whose rows are whole 16-byte words go to LDS directly (global_load_lds, no registers); any other pitch or width is loaded
 // into registers (unaligned 16-byte loads, the last word of a row element by element) and written from there.
 #include "elem.h"
@@ -69,13 +69,11 @@ __device__ __forceinline__ f16_t keep_z(float z) {
   return z > 0.f && h == (f16_t)0.f ? (f16_t)5.9604645e-8f : h;
 }
 
-constexpr int BM = 128, BN = 128, BK = 64, kThreads = 256;
+constexpr int BM = 128, BN = 128, BK = 64, kThreads = 256;    // tn_kernel's tile
 constexpr int kTileBytes = 128 * BK * 2;                      // one operand's stage
 constexpr int kStage = 2 * kTileBytes;
 
 __device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
-
-__device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t word) { return word ^ ((row >> 1) & 7); }
 
 // 16 bytes at any alignment; elements at and past `left` read as zero
 template <typename T>
@@ -106,9 +104,23 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+__device__ __forceinline__ uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
+
 __device__ __forceinline__ void lds_dma16(const void *src, void *dst) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
+
+// The same transfer in inline assembly, for kernels that keep several stages in flight: the compiler would wait for all of them before
+// every LDS read.  It has no result register; the kernel counts the transfers itself (wait_vm).  m0 needs one wait state before its use.
+// First form: an address per lane; second: a uniform base and an offset per lane, nothing to compute from stage to stage.
+__device__ __forceinline__ void lds_dma16_async(const void *src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma16_async(const void *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 struct GemmArgs {
   const void *A, *B;                        // [M, K], [N, K]
@@ -136,135 +148,348 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t 
   tn = in / rows;
 }
 
-// four loads per thread and operand fill a stage; thread t of pass i covers LDS word i * 256 + t, i.e. row (i * 256 + t) / 8
-template <typename T, bool DIRECT>
-struct Loader {
-  const T *base;                             // first row of the tile
-  int64_t ld;
-  uint32_t rows, K;                          // valid rows of the tile (>= 1), contraction length
-  uint4 reg[4];
+// a stage of an operand: ROWS rows of 64 elements (128 bytes: whole lines of the operand, eight 16-byte words); word w of row r sits at
+// w ^ ((r >> 1) & 7), so that the 16 lanes that read one word of 16 neighbouring rows hit all 64 banks
+__device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t word) { return word ^ ((row >> 1) & 7); }
 
-  __device__ __forceinline__ void start(uint32_t k0, char *lds) {
+template <typename T, int ROWS, int THREADS, bool DIRECT>
+struct KLoader {
+  static constexpr int P = ROWS * 8 / THREADS;
+  const char *base;                          // the tile's first row at the next stage's first column (uniform)
+  uint32_t off[P];                           // this thread's words from there, in bytes (the host keeps the pitch below 2^22 elements)
+  uint32_t k;                                // the stage's first column
+  uint32_t K;
+  uint4 reg[DIRECT ? 1 : P];
+
+  static __device__ __forceinline__ uint32_t col(int i) { const uint32_t w = i * THREADS + threadIdx.x; return swz(w >> 3, w & 7) * 8; }
+  __device__ __forceinline__ void init(const void *p, int64_t ld, uint32_t r0, uint32_t rows, uint32_t K_) {
+    base = static_cast<const char *>(p) + (int64_t)r0 * ld * 2;
+    k = 0; K = K_;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t w = i * kThreads + threadIdx.x, r = w >> 3, k = k0 + swz(r, w & 7) * 8;
-      const T *p = base + (int64_t)min(r, rows - 1) * ld + k;          // (rows past the end repeat the last: their products are not stored)
-      if (DIRECT) {
-        lds_dma16(k < K ? (const void *)p : (const void *)g_zero16, lds + (i * kThreads + (threadIdx.x & ~63u)) * 16);
-      } else {
-        reg[i] = load_word(p, (int)K - (int)k);
-      }
+    for (int i = 0; i < P; i++) {            // (rows past the end repeat the last one: their products are not stored)
+      const uint32_t r = (i * THREADS + threadIdx.x) >> 3;
+      off[i] = (min(r0 + r, rows - 1) - r0) * (uint32_t)ld * 2 + col(i) * 2;
     }
   }
-  __device__ __forceinline__ void finish(char *lds) {
-    if (!DIRECT) {
+  // transfer i of the next stage
+  __device__ __forceinline__ void send(int i, uint32_t lds) {
+    if (k + 64 <= K) lds_dma16_async(base, off[i], lds + i * THREADS * 16);
+    else lds_dma16_async(k + col(i) < K ? (const void *)(base + off[i]) : (const void *)g_zero16, lds + i * THREADS * 16);      // (K % 8 == 0)
+  }
+  __device__ __forceinline__ void next() { base += 128; k += 64; }
+  __device__ __forceinline__ void start(uint32_t lds) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(lds + (i * kThreads + threadIdx.x) * 16) = reg[i];
+    for (int i = 0; i < P; i++) {
+      if constexpr (DIRECT) send(i, lds);
+      else reg[i] = load_word(reinterpret_cast<const T *>(base + off[i]), (int)K - (int)(k + col(i)));
+    }
+    next();
+  }
+  __device__ __forceinline__ void finish(char *lds) {
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int i = 0; i < P; i++) *reinterpret_cast<uint4 *>(lds + (i * THREADS + threadIdx.x) * 16) = reg[i];
     }
   }
 };
 
-template <typename T, bool DIRECT>
-__global__ void __launch_bounds__(kThreads, 2) nt_kernel(GemmArgs a) {
-  typedef typename Frag<T>::v8 v8;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
-  uint32_t tm, tn;
-  tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
-  const uint32_t m0 = tm * BM, n0 = tn * BN, lane = lane_id(), wave = wave_id();
-  const uint32_t wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-  Loader<T, DIRECT> la, lb;
-  la.base = static_cast<const T *>(a.A) + (int64_t)m0 * a.lda; la.ld = a.lda; la.rows = min((uint32_t)BM, a.M - m0); la.K = a.K;
-  lb.base = static_cast<const T *>(a.B) + (int64_t)n0 * a.ldb; lb.ld = a.ldb; lb.rows = min((uint32_t)BN, a.N - n0); lb.K = a.K;
-  f32x16 acc[2][2];                          // [n half][m half]
+// the bias of eight neighbouring columns, `left` of which exist
+template <typename T>
+__device__ __forceinline__ void load_bias(const GemmArgs &a, uint32_t n, int left, float (&b)[8]) {
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int e = 0; e < 8; e++) b[e] = 0.f;
+  if (!a.bias) return;
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+  for (int e = 0; e < 8; e++)
+    if (e < left) b[e] = a.bias_f32 ? static_cast<const float *>(a.bias)[n + e] : (float)static_cast<const T *>(a.bias)[n + e];
+}
+
+template <int ACT>
+__device__ __forceinline__ void act8(float (&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-  const uint32_t steps = (a.K + BK - 1) / BK;
-  la.start(0, lds); lb.start(0, lds + kTileBytes);
-  la.finish(lds); lb.finish(lds + kTileBytes);
-  for (uint32_t s = 0; s < steps; s++) {
-    char *cur = lds + (s & 1) * kStage, *nxt = lds + ((s + 1) & 1) * kStage;
-    stage_barrier();                         // (and everybody has read the other stage)
-    v8 fa[2][4], fb[2][4];
+  for (int e = 0; e < 8; e++) v[e] = act16(ACT, v[e]);
+}
+
+// Eight neighbouring columns of one row: bias, activation, residual, store.  `left` of them exist.
+template <typename T>
+__device__ __forceinline__ void finish8(const GemmArgs &a, uint32_t m, uint32_t n, int left, float (&v)[8], const float (&b)[8], const uint4 &resw) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+  for (int e = 0; e < 8; e++) v[e] += b[e];
+  if (a.z) {                                 // (rows of z are padded to whole words)
+    Vec<f16_t, 8> zz;
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const uint32_t rm = wm + h * 32 + (lane & 31), rn = wn + h * 32 + (lane & 31), w = q * 2 + (lane >> 5);
-        fa[h][q] = *reinterpret_cast<const v8 *>(cur + rm * 128 + swz(rm, w) * 16);
-        fb[h][q] = *reinterpret_cast<const v8 *>(cur + kTileBytes + rn * 128 + swz(rn, w) * 16);
-      }
-    if (s + 1 < steps) { la.start((s + 1) * BK, nxt); lb.start((s + 1) * BK, nxt + kTileBytes); }
-#pragma unroll
-    for (int q = 0; q < 4; q++)
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) acc[i][j] = mma(fb[i][q], fa[j][q], acc[i][j]);
-    if (s + 1 < steps) { la.finish(nxt); lb.finish(nxt + kTileBytes); }
+    for (int e = 0; e < 8; e++) zz.v[e] = keep_z(v[e]);
+    *reinterpret_cast<Vec<f16_t, 8> *>(a.z + (int64_t)m * a.ldz + n) = zz;
   }
-  __syncthreads();
-  // epilogue: 32 rows x 64 columns of the wavefront at a time through its own corner of LDS, so that a lane handles eight neighbouring
-  // columns and eight lanes a 128-byte line of the output
-  constexpr int kPitch = 68;                 // floats
-  float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kPitch;
+  switch (a.act) {                           // (uniform: one branch per word, not per element)
+    case 1: act8<1>(v); break;
+    case 2: act8<2>(v); break;
+    case 3: act8<3>(v); break;
+    case 4: act8<4>(v); break;
+    case kActGelu: act8<kActGelu>(v); break;
+    case kActSilu: act8<kActSilu>(v); break;
+    default: break;
+  }
+  if (a.res) {
+    T rr[8];
+    __builtin_memcpy(rr, &resw, 16);
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+    for (int e = 0; e < 8; e++) v[e] += (float)rr[e];
+  }
+  T out[8];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+  for (int e = 0; e < 8; e++) out[e] = (T)v[e];
+  T *dst = static_cast<T *>(a.C) + (int64_t)m * a.ldc + n;
+  if (left == 8) {
+    __builtin_memcpy(dst, out, 16);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float4 v = make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
-        *reinterpret_cast<float4 *>(mine + (lane & 31) * kPitch + i * 32 + e * 8 + (lane >> 5) * 4) = v;
+    for (int e = 0; e < 7; e++)
+      if (e < left) dst[e] = out[e];
+  }
+}
+
+// Workgroups stay and walk tiles (id, id + gridDim.x, ...): the first stages of the next tile are on their way while the epilogue of
+// this one runs.
+template <typename T, int BM_, int BN_, int WM, int WN, int ST, int OCC, bool DIRECT>
+__global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int THREADS = WM * WN * 64, MI = BM_ / WM / 32, NI = BN_ / WN / 32;
+  constexpr int kA = BM_ * 128, kBoth = (BM_ + BN_) * 128;    // bytes of a stage
+  static_assert(BN_ / WN == 64 && NI == 2, "the epilogue's rows are 64 columns");
+  constexpr int kEpi = 16 * 64 * 4;                           // bytes of a wavefront's epilogue corner: 16 rows
+  __shared__ __attribute__((aligned(16))) char lds[ST * kBoth + WM * WN * kEpi];
+  const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wm = (wave % WM) * (BM_ / WM), wn = (wave / WM) * 64;
+  const uint32_t tiles = a.tiles_m * a.tiles_n, steps = (a.K + 63) / 64;
+  KLoader<T, BM_, THREADS, DIRECT> la;
+  KLoader<T, BN_, THREADS, DIRECT> lb;
+  constexpr int PER = decltype(la)::P + decltype(lb)::P;      // transfers per stage and thread
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 1024;
+  v8 fa[2][MI], fb[2][NI];                   // operands of two quarters of a stage
+  const uint32_t ra = wm + (lane & 31), rb = wn + (lane & 31);
+  auto read_quarter = [&](const char *cur, int q) {
+#pragma unroll
+    for (int h = 0; h < MI; h++) fa[q & 1][h] = *reinterpret_cast<const v8 *>(cur + (ra + h * 32) * 128 + swz(ra + h * 32, q * 2 + (lane >> 5)) * 16);
+#pragma unroll
+    for (int h = 0; h < NI; h++) fb[q & 1][h] = *reinterpret_cast<const v8 *>(cur + kA + (rb + h * 32) * 128 + swz(rb + h * 32, q * 2 + (lane >> 5)) * 16);
+  };
+  // what the loaders fetch next: stage `ls` of tile `lt`
+  uint32_t lt = blockIdx.x, ls = 0;
+  auto aim = [&]() {
+    uint32_t tm, tn;
+    tile_of(lt, a.tiles_m, a.tiles_n, tm, tn);
+    la.init(a.A, a.lda, tm * BM_, a.M, a.K);
+    lb.init(a.B, a.ldb, tn * BN_, a.N, a.K);
+  };
+  auto advance = [&]() {
+    la.next(); lb.next();
+    if (++ls == steps) {
+      ls = 0; lt += gridDim.x;
+      if (lt < tiles) aim();
+    }
+  };
+  // A ring of ST stages in LDS.  A quarter's operands are read while the quarter before it is multiplied.  The one barrier of a stage
+  // sits before its last quarter's products, when everybody has read that quarter: the stage's place is free again and the next stage
+  // is whole (the younger ones may stay on their way); the transfers of the stage ST ahead go out between the products.
+  uint32_t ahead = 0;                        // stages fetched and not yet finished with
+  if (lt < tiles) aim();
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int s = 0; s < ST; s++)
+      if (lt < tiles) {
+#pragma unroll
+        for (int t = 0; t < decltype(la)::P; t++) la.send(t, lds0 + s * kBoth);
+#pragma unroll
+        for (int t = 0; t < decltype(lb)::P; t++) lb.send(t, lds0 + s * kBoth + kA);
+        advance();
+        ahead++;
       }
-    wave_order();
+    if (ahead == ST) wait_vm<(ST - 1) * PER>();
+    else wait_vm<0>();
+    __syncthreads();
+    read_quarter(lds, 0);
+  }
+  uint32_t at = 0;                           // the stage's place in the ring
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    uint32_t tm, tn;
+    tile_of(tile, a.tiles_m, a.tiles_n, tm, tn);
+    const uint32_t m0 = tm * BM_, n0 = tn * BN_;
+    f32x16 acc[NI][MI];
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-      const uint32_t r = p * 8 + (lane >> 3), c = (lane & 7) * 8, m = m0 + wm + j * 32 + r, n = n0 + wn + c;
-      if (m < a.M && n < a.N) {
-        float v[8];
-        *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(mine + r * kPitch + c);
-        *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(mine + r * kPitch + c + 4);
-        const int left = min(8, (int)(a.N - n));
-        if (a.bias) {
+    for (int i = 0; i < NI; i++)
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (e < left) v[e] += a.bias_f32 ? static_cast<const float *>(a.bias)[n + e] : (float)static_cast<const T *>(a.bias)[n + e];
+      for (int j = 0; j < MI; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+    if constexpr (!DIRECT) {
+      la.init(a.A, a.lda, m0, a.M, a.K);
+      lb.init(a.B, a.ldb, n0, a.N, a.K);
+      la.start(0); lb.start(0);
+      __syncthreads();                       // (the tile before has been read)
+      at = 0;
+      la.finish(lds); lb.finish(lds + kA);
+      if (steps > 1) { la.start(0); lb.start(0); }
+      __syncthreads();
+      read_quarter(lds, 0);
+    }
+    for (uint32_t s = 0; s < steps; s++) {
+      const uint32_t nx = at + 1 == ST ? 0 : at + 1;
+#pragma unroll
+      for (int q = 0; q < 3; q++) {
+        read_quarter(lds + at * kBoth, q + 1);
+        if constexpr (!DIRECT) {
+          if (q == 0 && s + 1 < steps) {     // (the next stage's place was last read before the previous barrier)
+            la.finish(lds + nx * kBoth); lb.finish(lds + nx * kBoth + kA);
+            if (s + 2 < steps) { la.start(0); lb.start(0); }
+          }
         }
-        if (a.z) {                           // (rows of z are padded to whole words)
-          Vec<f16_t, 8> zz;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 8; e++) zz.v[e] = keep_z(v[e]);
-          *reinterpret_cast<Vec<f16_t, 8> *>(a.z + (int64_t)m * a.ldz + n) = zz;
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+          for (int j = 0; j < MI; j++) acc[i][j] = mma(fb[q & 1][i], fa[q & 1][j], acc[i][j]);
+      }
+      bool send = false;
+      if constexpr (DIRECT) {
+        if (ahead > 1) {                     // another stage follows, of this tile or the next
+          if (ahead == ST) wait_vm<(ST - 2) * PER>();
+          else wait_vm<0>();
+          __syncthreads();
+          read_quarter(lds + nx * kBoth, 0);
         }
-        if (a.act) {
+        __builtin_amdgcn_sched_barrier(0);
+        send = lt < tiles;
+      } else if (s + 1 < steps) {
+        __syncthreads();
+        read_quarter(lds + nx * kBoth, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const uint32_t to = lds0 + at * kBoth;
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] = act16(a.act, v[e]);
+      for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int j = 0; j < MI; j++) {
+          acc[i][j] = mma(fb[1][i], fa[1][j], acc[i][j]);
+          if constexpr (DIRECT) {
+            if (send) {
+              const int x = i * MI + j;
+#pragma unroll
+              for (int t = x * PER / (NI * MI); t < (x + 1) * PER / (NI * MI); t++) {
+                if (t < decltype(la)::P) la.send(t, to);
+                else lb.send(t - decltype(la)::P, to + kA);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         }
-        if (a.res) {
-          const uint4 w = load_word(static_cast<const T *>(a.res) + (int64_t)m * a.ldr + n, left);
-          T rr[8];
-          __builtin_memcpy(rr, &w, 16);
+      if constexpr (DIRECT) {
+        if (send) advance();
+        else ahead--;
+      }
+      at = nx;
+    }
+    // Epilogue: 16 rows of the wavefront's 64 columns at a time through its own corner of LDS (16-byte word w of row r at w ^ r), so
+    // that a lane handles eight neighbouring columns and eight lanes a 128-byte line of the output.  The passes stay a loop: unrolled
+    // over passes and activations the epilogue outgrows the instruction cache.
+    float *mine = reinterpret_cast<float *>(lds + ST * kBoth) + wave * 16 * 64;
+    const uint32_t er = lane >> 3, ec = lane & 7, n = n0 + wn + ec * 8;
+    const int left = min(8, (int)a.N - (int)n);
+    float b[8];
+    load_bias<T>(a, n, left, b);
+    uint32_t m = m0 + wm + er;               // this lane's next row
+    const T *res = static_cast<const T *>(a.res) + (int64_t)m * a.ldr + n;
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (a.res && m < a.M) next = load_word(res, left);
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] += (float)rr[e];
+    for (int j = 0; j < MI; j++) {
+#pragma unroll 1
+      for (uint32_t half = 0; half < 2; half++) {
+        if (((lane >> 4) & 1) == half) {
+#pragma unroll
+          for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              *reinterpret_cast<float4 *>(mine + (lane & 15) * 64 + ((i * 8 + e * 2 + (lane >> 5)) ^ (lane & 15)) * 4) =
+                  make_float4(acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]);
         }
-        T out[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) out[e] = (T)v[e];
-        T *dst = static_cast<T *>(a.C) + (int64_t)m * a.ldc + n;
-        if (left == 8) __builtin_memcpy(dst, out, 16);
-        else {
-#pragma unroll
-          for (int e = 0; e < 7; e++)
-            if (e < left) dst[e] = out[e];
+        wave_order();
+#pragma unroll 1
+        for (uint32_t p = 0; p < 16; p += 8, m += 8) {
+          const uint4 resw = next;
+          res += 8 * a.ldr;
+          if (a.res && m + 8 < a.M) next = load_word(res, left);       // (a pass ahead; past the wavefront's last row it is not used)
+          if (m < a.M && left > 0) {
+            const uint32_t r = p + er;
+            float v[8];
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2) ^ r) * 4);
+            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2 + 1) ^ r) * 4);
+            finish8<T>(a, m, n, left, v, b, resw);
+          }
         }
+        wave_order();
       }
     }
-    wave_order();
   }
+}
+
+// Few output tiles: 32 x 32 tiles, the contraction cut over the workgroup's eight wavefronts (step 16 w, 16 (w + 8), ...), their
+// products joined in LDS in wavefront order.  Operands go from memory to the product's registers: every word is used once.
+template <typename T, bool WORDS>
+__global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int kPitch = 36;
+  __shared__ __attribute__((aligned(16))) float part[8][32 * kPitch];
+  const uint32_t tm = blockIdx.x % a.tiles_m, tn = blockIdx.x / a.tiles_m, m0 = tm * 32, n0 = tn * 32;
+  const uint32_t lane = lane_id(), wave = wave_id(), r = lane & 31;
+  const T *pa = static_cast<const T *>(a.A) + (int64_t)min(m0 + r, a.M - 1) * a.lda;
+  const T *pb = static_cast<const T *>(a.B) + (int64_t)min(n0 + r, a.N - 1) * a.ldb;
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; e++) acc[e] = 0.f;
+  constexpr int U = 4;                       // steps whose loads are in flight together
+  for (uint32_t k0 = wave * 16; k0 < a.K; k0 += 8 * 16 * U) {
+    uint4 wa[U], wb[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
+      if (WORDS) {
+        const bool in = k < a.K;
+        wa[u] = in ? *reinterpret_cast<const uint4 *>(pa + k) : make_uint4(0, 0, 0, 0);
+        wb[u] = in ? *reinterpret_cast<const uint4 *>(pb + k) : make_uint4(0, 0, 0, 0);
+      } else {
+        wa[u] = load_word(pa + k, (int)a.K - (int)k);
+        wb[u] = load_word(pb + k, (int)a.K - (int)k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      v8 fa, fb;
+      __builtin_memcpy(&fa, &wa[u], 16);
+      __builtin_memcpy(&fb, &wb[u], 16);
+      acc = mma(fb, fa, acc);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    *reinterpret_cast<float4 *>(&part[wave][r * kPitch + e * 8 + (lane >> 5) * 4]) = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+  __syncthreads();
+  if (threadIdx.x >= 128) return;            // 32 rows x four words
+  const uint32_t er = threadIdx.x >> 2, ec = (threadIdx.x & 3) * 8, m = m0 + er, n = n0 + ec;
+  if (m >= a.M || n >= a.N) return;
+  const int left = min(8, (int)a.N - (int)n);
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; w++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += part[w][er * kPitch + ec + e];
+  uint4 resw = make_uint4(0, 0, 0, 0);
+  if (a.res) resw = load_word(static_cast<const T *>(a.res) + (int64_t)m * a.ldr + n, left);
+  float b[8];
+  load_bias<T>(a, n, left, b);
+  finish8<T>(a, m, n, left, v, b, resw);
 }
 
 // ------------------------------------------------------------------------------------------------ dz^T x
@@ -480,13 +705,30 @@ BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K) {
 
 bool dtype16(int d) { return d == SL_BF16 || d == SL_F16; }
 
+template <typename T, int BM_, int BN_, int WM, int WN, int ST, int OCC, int PERCU>
+void nt_tiles(GemmArgs a, bool direct, hipStream_t st) {
+  a.tiles_m = (a.M + BM_ - 1) / BM_; a.tiles_n = (a.N + BN_ - 1) / BN_;
+  const uint32_t tiles = a.tiles_m * a.tiles_n, most = 256 * PERCU;       // (a multiple of eight: a workgroup stays on its XCD's tiles)
+  const dim3 g(tiles < most ? tiles : most), b(WM * WN * 64);
+  if (direct) hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, ST, OCC, true>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), g, b, 0, st, a);
+}
+
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
-  a.tiles_m = (a.M + BM - 1) / BM; a.tiles_n = (a.N + BN - 1) / BN;
-  const dim3 g(a.tiles_m * a.tiles_n), b(kThreads);
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);
-  if (direct) hipLaunchKernelGGL((nt_kernel<T, true>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((nt_kernel<T, false>), g, b, 0, st, a);
+  const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
+  // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches are rare and take the other)
+  if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22)) {
+    a.tiles_m = (a.M + 31) / 32; a.tiles_n = (a.N + 31) / 32;
+    const dim3 g(a.tiles_m * a.tiles_n), b(512);
+    if (direct) hipLaunchKernelGGL((nt_few_kernel<T, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((nt_few_kernel<T, false>), g, b, 0, st, a);
+  } else if (direct && tiles >= 1024 && a.K >= 512 && a.N >= 256) {
+    nt_tiles<T, 256, 256, 2, 4, 2, 2, 1>(a, direct, st);
+  } else {
+    nt_tiles<T, 128, 128, 2, 2, 2, 2, 2>(a, direct, st);
+  }
 }
 
 template <typename T>
