@@ -949,16 +949,17 @@ int sl_layer_norm_bwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, cons
 int sl_dropout(int dtype, const void *d_x, int64_t ldx, const void *d_res, int64_t ldr, uint64_t n, uint32_t F, float p, uint64_t seed,
                const int64_t *d_seed, void *d_y, int64_t ldy, void *stream);
 /* y = act(x W^T + bias) + res: x [M, K], W [N, K], res and y [M, N] in bf16 or fp16, bias [N] in that type or fp32; bias / res may be
- * NULL.  act: 0 identity, 1 relu, 2 elu, 3 tanh, 4 leakyrelu(0.2), 5 gelu, 6 silu.  d_z (may be NULL): the pre-activations in fp16,
- * pitch ldz a multiple of 8 and 16-byte aligned, for the backward pass. */
+ * NULL.  act: 0 identity, 1 relu, 2 elu, 3 tanh, 4 leakyrelu(0.2), 5 gelu, 6 silu.  d_kept (may be NULL): sl_linear16_kept_bytes(act, M, N)
+ * bytes, 16-byte aligned, for the backward pass of an activation: one bit of every pre-activation (relu, leakyrelu) or its fp16 value. */
+size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N);
 int sl_linear16_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, int bias_f32, const void *d_res,
-                    int64_t ldr, uint32_t M, uint32_t N, uint32_t K, int act, void *d_y, int64_t ldy, void *d_z, int64_t ldz, void *stream);
-/* dx [M, K], dW [N, K], db [N] (each may be NULL; db only together with dW) from dy and d_z (act != 0; pitch: N rounded up to 8).
+                    int64_t ldr, uint32_t M, uint32_t N, uint32_t K, int act, void *d_y, int64_t ldy, void *d_kept, void *stream);
+/* dx [M, K], dW [N, K], db [N] (each may be NULL; db only together with dW) from dy and d_kept (act != 0).  d_scratch: 16-byte aligned.
  * The rows of dz^T x are cut into slices whose products are added in slice order (no atomics). */
 size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K);
-int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy, const void *d_z,
-                    int64_t ldz, uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, void *d_db,
-                    int db_f32, void *d_scratch, void *stream);
+int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy, const void *d_kept,
+                    uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, void *d_db, int db_f32,
+                    void *d_scratch, void *stream);
 /* Rows of C logits with a label each (int32 or int64; < 0: no label, log probability 0; >= C: NaN): log probability of the label,
  * entropy of the softmax, and the k <= min(C, 64) largest logits' log probabilities and indices (value descending, lowest index first,
  * NaN on top).  A logit of -inf has probability 0; a row without a finite logit answers -inf, entropy 0 and has gradient 0; +inf or

@@ -269,9 +269,10 @@ SIGNATURES = {
     "sl_layer_norm_bwd": (C.c_int, [C.c_int, C.c_int, _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_uint32, C.c_uint32, _P, C.c_int64, _P, _P, _P, _P]),
     "sl_dropout": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, C.c_uint64, C.c_uint32, C.c_float, C.c_uint64, _P, _P, C.c_int64, _P]),
     "sl_linear16_fwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
-                                  _P, C.c_int64, _P, C.c_int64, _P]),
+                                  _P, C.c_int64, _P, _P]),
+    "sl_linear16_kept_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32]),
     "sl_linear16_bwd_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
-    "sl_linear16_bwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+    "sl_linear16_bwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
                                   _P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, _P]),
     "sl_label_logprobs_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
     "sl_label_logprobs_fwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P, _P, _P]),

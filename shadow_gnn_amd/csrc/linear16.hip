@@ -62,11 +62,42 @@ __device__ __forceinline__ float slope16(int act, float z) {
     default: return 1.f;
   }
 }
-// The pre-activation is kept for the backward pass in fp16 whatever the operands' type: eleven bits keep act'(z) well inside a bf16
-// step, and where fp16's range ends every activation's slope has reached its limit.  A tiny positive z keeps its sign (relu's slope).
-__device__ __forceinline__ f16_t keep_z(float z) {
-  const f16_t h = (f16_t)z;
-  return z > 0.f && h == (f16_t)0.f ? (f16_t)5.9604645e-8f : h;
+// What the forward pass keeps of z for the backward pass.  relu and leakyrelu: one bit (z > 0), a byte per eight columns.  The others:
+// z in fp16 whatever the operands' type -- eleven bits keep act'(z) well inside a bf16 step, and where fp16's range ends every slope
+// has reached its limit.
+__host__ __device__ constexpr bool keeps_bits(int act) { return act == 1 || act == 4; }
+__host__ __device__ constexpr uint64_t up(uint64_t v, uint64_t m) { return (v + m - 1) / m * m; }
+// bytes of a kept row: whole 16-byte words
+__host__ __device__ constexpr uint64_t kept_pitch(int act, uint32_t N) { return keeps_bits(act) ? up((N + 7) / 8, 16) : up(N, 8) * 2; }
+
+// eight elements of dz = dy act'(z), rounded to the operands' type (the products need 16-bit operands; for relu nothing is lost).
+// z: the word of kept values, or the byte of kept bits in z.x.  A dy of zero is a dz of zero.
+template <typename T>
+__device__ __forceinline__ uint4 dz_word(int act, const uint4 &dy, const uint4 &z) {
+  uint4 out;
+  if (act == 1) {
+    const uint32_t in[4] = {dy.x, dy.y, dy.z, dy.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {            // bits 2 q and 2 q + 1 of the byte as masks of the two halves
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)z.x, 2 * q, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)z.x, 2 * q + 1, 1);
+      o[q] = in[q] & ((lo & 0xFFFFu) | (hi & 0xFFFF0000u));
+    }
+    out = make_uint4(o[0], o[1], o[2], o[3]);
+  } else {
+    T g[8], r[8];
+    f16_t zz[8];
+    __builtin_memcpy(g, &dy, 16);
+    __builtin_memcpy(zz, &z, 16);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float slope = act == 4 ? ((z.x >> e) & 1u ? 1.f : 0.2f) : slope16(act, (float)zz[e]);
+      const float v = (float)g[e];
+      r[e] = (T)(v == 0.f ? 0.f : v * slope);
+    }
+    __builtin_memcpy(&out, r, 16);
+  }
+  return out;
 }
 
 constexpr int BM = 128, BN = 128, BK = 64, kThreads = 256;    // tn_kernel's tile
@@ -132,8 +163,7 @@ struct GemmArgs {
   int64_t ldr;
   void *C;
   int64_t ldc;
-  f16_t *z;
-  int64_t ldz;
+  char *kept;                                // kept_pitch(act, N) bytes a row; null: nothing is kept
   int act;
   uint32_t tiles_m, tiles_n;
 };
@@ -210,16 +240,28 @@ __device__ __forceinline__ void act8(float (&v)[8]) {
   for (int e = 0; e < 8; e++) v[e] = act16(ACT, v[e]);
 }
 
-// Eight neighbouring columns of one row: bias, activation, residual, store.  `left` of them exist.
+// Eight neighbouring columns of one row: bias, activation, residual, store.  `left` of them exist.  lds_bits: where kept bits are
+// gathered instead of stored.
 template <typename T>
-__device__ __forceinline__ void finish8(const GemmArgs &a, uint32_t m, uint32_t n, int left, float (&v)[8], const float (&b)[8], const uint4 &resw) {
+__device__ __forceinline__ void finish8(const GemmArgs &a, uint32_t m, uint32_t n, int left, float (&v)[8], const float (&b)[8], const uint4 &resw,
+                                        uint8_t *lds_bits = nullptr) {
 #pragma unroll
   for (int e = 0; e < 8; e++) v[e] += b[e];
-  if (a.z) {                                 // (rows of z are padded to whole words)
-    Vec<f16_t, 8> zz;
+  if (a.kept) {
+    char *row = a.kept + (uint64_t)m * kept_pitch(a.act, a.N);
+    if (keeps_bits(a.act)) {
+      uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) zz.v[e] = keep_z(v[e]);
-    *reinterpret_cast<Vec<f16_t, 8> *>(a.z + (int64_t)m * a.ldz + n) = zz;
+      for (int e = 0; e < 8; e++) bits |= v[e] > 0.f ? 1u << e : 0u;
+      if (left < 8) bits &= (1u << left) - 1u;
+      if (lds_bits) *lds_bits = (uint8_t)bits;
+      else row[n / 8] = (char)bits;
+    } else {
+      Vec<f16_t, 8> zz;
+#pragma unroll
+      for (int e = 0; e < 8; e++) zz.v[e] = (f16_t)v[e];
+      *reinterpret_cast<Vec<f16_t, 8> *>(row + n * 2) = zz;
+    }
   }
   switch (a.act) {                           // (uniform: one branch per word, not per element)
     case 1: act8<1>(v); break;
@@ -492,6 +534,172 @@ __global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
   finish8<T>(a, m, n, left, v, b, resw);
 }
 
+// ------------------------------------------------------------------------------------------------ tall, narrow products
+// N <= 256 and K <= 256 (the hidden widths of the graph models) over many rows are bound by memory: x, res and y cross it once.  The
+// weight stays in the registers of NWC wavefronts (32 output columns each) for the whole launch; four more wavefronts do nothing but
+// send 32-row tiles of A, and of what else the rows need (SIDE), to a ring of RS places in LDS.  Transfers are counted together with a
+// wavefront's own loads and stores and in order: apart from each other, the senders keep RS - 1 tiles on their way and the multiplying
+// wavefronts never wait for their stores (with the residual loaded by them the forward pass took 140, dx 150 us at 289127 x 256 x 256).
+// One barrier per tile: the tile is whole, and the one before it has been read.
+//   SIDE 1: the residual's rows.
+//   SIDE 2, 3 (dx = dz W; A is dy): kept fp16 values / kept bits.  The tile becomes dz = dy act'(z) in place, each wavefront a share
+//   of it, and is stored for dz^T x if asked for; a second barrier then.
+// Bits kept by the forward pass are gathered in LDS and leave a tile later as whole words (as bytes they cost 25 us of 140).
+struct NarrowArgs {
+  GemmArgs g;
+  int b_cols;                                // 1: B is given as [K, N] (pitch ldb)
+  const char *kept;                          // SIDE 2, 3: kept values of g.K columns
+  int kept_act;
+  void *dz;                                  // SIDE 2, 3: null, or where dz goes, pitch lddz
+  int64_t lddz;
+};
+
+template <int W>                             // W 16-byte words per row
+__device__ __forceinline__ uint32_t swz_row(uint32_t row, uint32_t word) { return W >= 16 ? word ^ (row & 15) : word ^ ((row >> 1) & 7); }
+
+template <typename T, int NWC, int KS, int RS, int SIDE>
+__global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int R = 32, W = KS * 2, WS = SIDE == 1 ? NWC * 4 : SIDE == 2 ? W : 0;      // rows of a tile, words of its rows and of the side's
+  constexpr int kA = R * W * 16, kSide = SIDE == 3 ? R * 32 : R * WS * 16, kPlace = kA + kSide;
+  constexpr int PA = R * W / 256, PS = SIDE == 3 ? 1 : R * WS / 256, PER = PA + PS;    // transfers per tile and lane
+  __shared__ __attribute__((aligned(16))) char lds[RS * kPlace + NWC * 2048 + (SIDE < 2 ? 2 * R * 32 : 0)];
+  const GemmArgs &a = n.g;
+  const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = (a.M + R - 1) / R;
+  const bool bits_out = SIDE < 2 && a.kept && keeps_bits(a.act);
+  if (wave >= NWC) {                         // ---- the sending wavefronts
+    const uint32_t me = wave - NWC, lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+    const uint32_t kw = (uint32_t)(kept_pitch(1, a.K) / 16);           // SIDE 3: words of a row of bits (1 or 2)
+    auto send = [&](uint32_t tile, uint32_t slot) {
+      const uint32_t place = lds0 + slot * kPlace + me * 1024;
+#pragma unroll
+      for (int i = 0; i < PA; i++) {
+        const uint32_t w = (i * 4 + me) * 64 + lane, r = w / W, k = swz_row<W>(r, w % W) * 8, row = min(tile * R + r, a.M - 1);
+        const T *p = static_cast<const T *>(a.A) + (int64_t)row * a.lda + k;
+        lds_dma16_async(k < a.K ? (const void *)p : (const void *)g_zero16, place + i * 4096);
+      }
+      if constexpr (SIDE == 1 || SIDE == 2) {
+        const char *base = SIDE == 1 ? static_cast<const char *>(a.res) : n.kept;
+        const int64_t pitch = SIDE == 1 ? a.ldr * 2 : (int64_t)kept_pitch(5, a.K);
+        const uint32_t width = SIDE == 1 ? a.N : a.K;
+#pragma unroll
+        for (int i = 0; i < PS; i++) {
+          const uint32_t w = (i * 4 + me) * 64 + lane, r = w / WS, k = swz_row<WS>(r, w % WS) * 8, row = min(tile * R + r, a.M - 1);
+          lds_dma16_async(k < width ? (const void *)(base + row * pitch + k * 2) : (const void *)g_zero16, place + kA + i * 4096);
+        }
+      }
+      if constexpr (SIDE == 3) {
+        if (lane < 16) {                     // (64 words, 16 of each sender)
+          const uint32_t w = me * 16 + lane, row = min(tile * R + w / kw, a.M - 1);
+          lds_dma16_async(w < R * kw ? (const void *)(n.kept + (uint64_t)row * kw * 16 + (w % kw) * 16) : (const void *)g_zero16, lds0 + slot * kPlace + kA + me * 256);
+        }
+      }
+    };
+    uint32_t next = blockIdx.x, slot = 0;    // the tile and place sent next
+    for (int s = 0; s < RS - 1; s++)
+      if (next < tiles) { send(next, slot); next += gridDim.x; slot++; }
+    uint32_t left = slot;                    // tiles sent and not yet awaited
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      if (left == RS - 1) wait_vm<(RS - 2) * PER>();
+      else wait_vm<0>();
+      left--;
+      __syncthreads();
+      if (SIDE >= 2) __syncthreads();
+      if (next < tiles) { send(next, slot); next += gridDim.x; left++; slot = slot + 1 == RS ? 0 : slot + 1; }
+    }
+    if (bits_out) __syncthreads();
+    return;
+  }
+  // ---- the multiplying wavefronts
+  const uint32_t n0 = wave * 32;
+  v8 fb[KS];                                 // B's rows n0 + (lane & 31): the step's eight elements of this lane
+  {
+    const uint32_t row = min(n0 + (lane & 31), a.N - 1);
+#pragma unroll
+    for (int q = 0; q < KS; q++) {
+      const uint32_t k = q * 16 + (lane >> 5) * 8;
+      if (n.b_cols) {
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = k + j < a.K ? static_cast<const T *>(a.B)[(int64_t)(k + j) * a.ldb + row] : (T)0.f;
+        __builtin_memcpy(&fb[q], e, 16);
+      } else {
+        const uint4 w = load_word(static_cast<const T *>(a.B) + (int64_t)row * a.ldb + k, (int)a.K - (int)k);
+        __builtin_memcpy(&fb[q], &w, 16);
+      }
+    }
+  }
+  float *mine = reinterpret_cast<float *>(lds + RS * kPlace) + wave * 512;             // 16 rows of 32 columns
+  uint8_t *bits = reinterpret_cast<uint8_t *>(lds + RS * kPlace + NWC * 2048);         // two tiles of R rows, 32 bytes each
+  const uint32_t er = lane >> 2, ec = lane & 3, col = n0 + ec * 8;
+  const int left = min(8, (int)a.N - (int)col);
+  float b[8];
+  load_bias<T>(a, col, left, b);
+  const uint32_t bw = (uint32_t)(kept_pitch(1, a.N) / 16);             // words of an output row of bits (1 or 2)
+  auto flush_bits = [&](uint32_t tile, uint32_t which) {               // R rows x bw words, by the first wavefront
+    const uint32_t w = threadIdx.x, r = w / bw, m = tile * R + r;
+    if (w < R * bw && m < a.M) *reinterpret_cast<uint4 *>(a.kept + ((uint64_t)m * bw + w % bw) * 16) = *reinterpret_cast<const uint4 *>(bits + (which * R + r) * 32 + (w % bw) * 16);
+  };
+  if (bits_out) {                            // (columns past N: no bits)
+    for (uint32_t w = threadIdx.x; w < 2 * R * 8; w += NWC * 64) reinterpret_cast<uint32_t *>(bits)[w] = 0;
+  }
+  uint32_t at = 0, turn = 0;
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+    char *cur = lds + at * kPlace;
+    at = at + 1 == RS ? 0 : at + 1;
+    __syncthreads();
+    const uint32_t m0 = tile * R;
+    if (bits_out && tile != blockIdx.x) flush_bits(tile - gridDim.x, turn ^ 1);
+    if constexpr (SIDE >= 2) {
+#pragma unroll
+      for (int i = 0; i < R * W / (NWC * 64); i++) {
+        const uint32_t w = i * NWC * 64 + threadIdx.x, r = w / W, c = w % W;
+        uint4 *p = reinterpret_cast<uint4 *>(cur + (r * W + swz_row<W>(r, c)) * 16);
+        uint4 z = make_uint4(0, 0, 0, 0);
+        if constexpr (SIDE == 2) z = *reinterpret_cast<const uint4 *>(cur + kA + (r * W + swz_row<W>(r, c)) * 16);
+        else if (c * 8 < a.K) z.x = *reinterpret_cast<const uint8_t *>(cur + kA + r * (kept_pitch(1, a.K)) + c);
+        const uint4 d = dz_word<T>(n.kept_act, *p, z);
+        *p = d;
+        if (n.dz && m0 + r < a.M && c * 8 < a.K) *reinterpret_cast<uint4 *>(static_cast<T *>(n.dz) + (int64_t)(m0 + r) * n.lddz + c * 8) = d;
+      }
+      __syncthreads();
+    }
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    const uint32_t ra = lane & 31;
+#pragma unroll
+    for (int q = 0; q < KS; q++) acc = mma(fb[q], *reinterpret_cast<const v8 *>(cur + (ra * W + swz_row<W>(ra, q * 2 + (lane >> 5))) * 16), acc);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {       // 16 rows at a time through this wavefront's corner (word w of row r at w ^ ((r >> 1) & 7))
+      if (((lane >> 4) & 1) == h) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          *reinterpret_cast<float4 *>(mine + (lane & 15) * 32 + swz(lane & 15, e * 2 + (lane >> 5)) * 4) =
+              make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+      }
+      wave_order();
+      const uint32_t r = h * 16 + er, m = m0 + r;
+      if (m < a.M && left > 0) {
+        float v[8];
+        *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(mine + er * 32 + swz(er, ec * 2) * 4);
+        *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(mine + er * 32 + swz(er, ec * 2 + 1) * 4);
+        uint4 resw = make_uint4(0, 0, 0, 0);
+        if constexpr (SIDE == 1) resw = *reinterpret_cast<const uint4 *>(cur + kA + (r * WS + swz_row<WS>(r, wave * 4 + ec)) * 16);
+        finish8<T>(a, m, col, left, v, b, resw, bits_out ? bits + (turn * R + r) * 32 + col / 8 : nullptr);
+      }
+      wave_order();
+    }
+  }
+  if (bits_out) {
+    __syncthreads();
+    // (the last tile: the largest that this workgroup walks)
+    const uint32_t last = blockIdx.x + (tiles - 1 - blockIdx.x) / gridDim.x * gridDim.x;
+    flush_bits(last, turn ^ 1);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ dz^T x
 struct TnArgs {
   const void *A, *B;                        // dz [M, N], x [M, K]
@@ -533,7 +741,7 @@ struct RowLoader {
 
 // eight consecutive rows k .. k + 7 of column c0 + (lane & 15), as a product's operand: two transposing reads of four rows each (lane
 // 4 q + p of a group of 16 points at 8-byte piece p of row q; it receives column (lane & 15) of the four rows)
-template <typename T>
+template <typename T, int W>
 __device__ __forceinline__ typename Frag<T>::v8 read_cols(const char *img, uint32_t k, uint32_t c0) {
   const uint32_t l = lane_id() & 15, r = l >> 2, p = l & 3;
   typedef short s4 __attribute__((ext_vector_type(4)));
@@ -541,7 +749,7 @@ __device__ __forceinline__ typename Frag<T>::v8 read_cols(const char *img, uint3
 #pragma unroll
   for (int t = 0; t < 2; t++) {
     const uint32_t row = k + 4 * t + r, word = (c0 >> 3) + (p >> 1);
-    const char *at = img + row * 256 + swz_t(row, word) * 16 + (p & 1) * 8;
+    const char *at = img + (row * W + swz_t(row, word)) * 16 + (p & 1) * 8;
     u.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
   }
   return u.v;
@@ -585,8 +793,8 @@ __global__ void __launch_bounds__(kThreads, 2) tn_kernel(TnArgs a) {
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const uint32_t kk = q * 16 + (lane >> 5) * 8, half = ((lane >> 4) & 1) * 16;
-        fa[h][q] = read_cols<T>(cur, kk, wn + h * 32 + half);
-        fb[h][q] = read_cols<T>(cur + kTileBytes, kk, wk + h * 32 + half);
+        fa[h][q] = read_cols<T, 16>(cur, kk, wn + h * 32 + half);
+        fb[h][q] = read_cols<T, 16>(cur + kTileBytes, kk, wk + h * 32 + half);
       }
     if (s + 1 < steps) { la.start(r0 + (s + 1) * BK, r1, nxt); lb.start(r0 + (s + 1) * BK, r1, nxt + kTileBytes); }
 #pragma unroll
@@ -621,44 +829,151 @@ __global__ void __launch_bounds__(kThreads, 2) tn_kernel(TnArgs a) {
   }
 }
 
-// sums of the slices in slice order
-template <typename T>
-__global__ void __launch_bounds__(256) tn_join_kernel(const float *__restrict__ part, uint32_t slices, uint32_t N, uint32_t K, T *C, int64_t ldc) {
-  const uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x, total = (uint64_t)N * K;
-  if (e >= total) return;
-  float t = 0.f;
-#pragma unroll 8
-  for (uint32_t s = 0; s < slices; s++) t += part[s * total + e];
-  C[(int64_t)(e / K) * ldc + e % K] = (T)t;
+// dz^T x of narrow operands (N <= 128 NB, K <= 64 KB): one workgroup holds all of dW -- 128 x 64 per wavefront -- and walks one row
+// slice, 32 rows a stage, both operands read once.  BITS: A is dy and its stage is masked in place by relu's (leakyrelu's) kept bits.
+// db: dz^T 1 on the same products, the 32-column groups of a 128-column block dealt to the block's KB wavefronts.
+struct TnNarrowArgs {
+  TnArgs t;
+  const char *kept;
+  int kept_act;
+};
+
+template <typename T, int NB, int KB, int RS, bool BITS>
+__global__ void __launch_bounds__(NB * KB * 64, 2) tn_narrow_kernel(TnNarrowArgs n) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int THREADS = NB * KB * 64, WA = NB * 16, WB = KB * 8;   // words of a row of dz and of x
+  constexpr int kA = 32 * WA * 16, kB = 32 * WB * 16, kM = BITS ? 1024 : 0, kBoth = kA + kB + kM;
+  constexpr int PA = 32 * WA / THREADS, PB = 32 * WB / THREADS, PER = PA + PB + (BITS ? 1 : 0), NJ = 4 / KB;
+  static_assert(PA >= 1 && PB >= 1, "whole transfers");
+  __shared__ __attribute__((aligned(16))) char lds[RS * kBoth];
+  const TnArgs &a = n.t;
+  const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave / KB, wk = wave % KB;
+  const uint32_t r0 = blockIdx.x * a.per, r1 = min(a.M, r0 + a.per);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + wave * 1024, ldsm = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + kA + kB;
+  const uint32_t kw = (uint32_t)(kept_pitch(1, a.N) / 16);           // words of a row of kept bits (1 or 2)
+  auto send = [&](uint32_t row, uint32_t slot) {
+#pragma unroll
+    for (int i = 0; i < PA; i++) {
+      const uint32_t w = i * THREADS + threadIdx.x, r = w / WA, c = swz_t(r, w % WA) * 8;
+      const T *p = static_cast<const T *>(a.A) + (int64_t)(row + r) * a.lda + c;
+      lds_dma16_async(row + r < r1 && c < a.N ? (const void *)p : (const void *)g_zero16, lds0 + slot * kBoth + i * THREADS * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; i++) {
+      const uint32_t w = i * THREADS + threadIdx.x, r = w / WB, c = swz_t(r, w % WB) * 8;
+      const T *p = static_cast<const T *>(a.B) + (int64_t)(row + r) * a.ldb + c;
+      lds_dma16_async(row + r < r1 && c < a.K ? (const void *)p : (const void *)g_zero16, lds0 + slot * kBoth + kA + i * THREADS * 16);
+    }
+    if constexpr (BITS) {                    // (every wavefront sends the same 64 words: one count of transfers for all)
+      const uint32_t r = lane / kw;
+      const char *p = n.kept + (uint64_t)(row + r) * kw * 16 + (lane % kw) * 16;
+      lds_dma16_async(r < 32 && row + r < r1 ? (const void *)p : (const void *)g_zero16, ldsm + slot * kBoth);
+    }
+  };
+  f32x16 acc[4][2], accb[NJ];                // [n][k] 32 x 32 blocks
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i][0][e] = acc[i][1][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NJ; i++) accb[i][e] = 0.f;
+  }
+  v8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; j++) ones[j] = (T)1.0f;
+  uint32_t next = r0, slot = 0;
+  for (int s = 0; s < RS - 1; s++)
+    if (next < r1) { send(next, slot); next += 32; slot++; }
+  uint32_t left = slot, at = 0;
+  for (uint32_t row = r0; row < r1; row += 32) {
+    if (left == RS - 1) wait_vm<(RS - 2) * PER>();
+    else wait_vm<0>();
+    left--;
+    __syncthreads();                         // the stage is whole, the one before it has been read
+    char *cur = lds + at * kBoth;
+    at = at + 1 == RS ? 0 : at + 1;
+    if (next < r1) { send(next, slot); next += 32; left++; slot = slot + 1 == RS ? 0 : slot + 1; }
+    if constexpr (BITS) {
+#pragma unroll
+      for (int i = 0; i < PA; i++) {
+        const uint32_t w = i * THREADS + threadIdx.x, r = w / WA, c = w % WA;
+        uint4 *p = reinterpret_cast<uint4 *>(cur + (r * WA + swz_t(r, c)) * 16);
+        const uint32_t bits = c * 8 < a.N ? *reinterpret_cast<const uint8_t *>(cur + kA + kB + r * kw * 16 + c) : 0u;
+        *p = dz_word<T>(n.kept_act, *p, make_uint4(bits, 0, 0, 0));
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const uint32_t kk = q * 16 + (lane >> 5) * 8, half = ((lane >> 4) & 1) * 16;
+      v8 fa[4], fb[2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) fa[i] = read_cols<T, WA>(cur, kk, wn * 128 + i * 32 + half);
+#pragma unroll
+      for (int j = 0; j < 2; j++) fb[j] = read_cols<T, WB>(cur + kA, kk, wk * 64 + j * 32 + half);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = mma(fa[i], fb[j], acc[i][j]);
+      if (a.part_b) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)          // (a wavefront-uniform choice among registers: four branches)
+          if (wk == (uint32_t)(i % KB)) accb[i / KB] = mma(fa[i], ones, accb[i / KB]);
+      }
+    }
+  }
+  // a lane holds column k = lane & 31: 128-byte lines of the partial product
+  float *part = a.part + (uint64_t)blockIdx.x * a.N * a.K;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const uint32_t r = wn * 128 + i * 32 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
+      if (r >= a.N) continue;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint32_t k = wk * 64 + j * 32 + (lane & 31);
+        if (k < a.K) part[(uint64_t)r * a.K + k] = acc[i][j][e];
+      }
+      if (a.part_b && wk == (uint32_t)(i % KB) && (lane & 31) == 0) a.part_b[(uint64_t)blockIdx.x * a.N + r] = accb[i / KB][e];
+    }
 }
+
+// sums of the slices in slice order: the first N K threads dW (part null: it is written already), N more db (part_b null: not wanted)
 template <typename T>
-__global__ void __launch_bounds__(256) bias_join_kernel(const float *__restrict__ part, uint32_t slices, uint32_t N, void *db, int db_f32) {
-  const uint32_t n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+__global__ void __launch_bounds__(256) tn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_b, uint32_t slices, uint32_t N,
+                                                      uint32_t K, T *C, int64_t ldc, void *db, int db_f32) {
+  const uint64_t total = part ? (uint64_t)N * K : 0;
+  uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   float t = 0.f;
+  if (e < total) {
 #pragma unroll 8
-  for (uint32_t s = 0; s < slices; s++) t += part[(uint64_t)s * N + n];
-  if (db_f32) static_cast<float *>(db)[n] = t;
-  else static_cast<T *>(db)[n] = (T)t;
+    for (uint32_t s = 0; s < slices; s++) t += part[s * total + e];
+    C[(int64_t)(e / K) * ldc + e % K] = (T)t;
+    return;
+  }
+  e -= total;
+  if (!part_b || e >= N) return;
+#pragma unroll 8
+  for (uint32_t s = 0; s < slices; s++) t += part_b[(uint64_t)s * N + e];
+  if (db_f32) static_cast<float *>(db)[e] = t;
+  else static_cast<T *>(db)[e] = (T)t;
 }
 
 // ------------------------------------------------------------------------------------------------ elementwise pieces
-// dz = dy act'(z), rounded to the operands' type (the products need 16-bit operands); pad columns are zero
+// dz = dy act'(z) of every word; pad columns are zero
 template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, const f16_t *z, T *dz, int64_t ld, uint32_t M, uint32_t N, int act) {
+__global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, const char *kept, T *dz, int64_t ld, uint32_t M, uint32_t N, int act) {
   const uint32_t words = (uint32_t)(ld / 8);
-  const uint64_t total = (uint64_t)M * words;
+  const uint64_t total = (uint64_t)M * words, pitch = kept_pitch(act, N);
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
     const uint64_t m = i / words;
-    const uint32_t n = (uint32_t)(i % words) * 8;
-    const uint4 w = load_word(dy + (int64_t)m * lddy + n, (int)N - (int)n);
-    T g[8];
-    __builtin_memcpy(g, &w, 16);
-    const Vec<f16_t, 8> zz = *reinterpret_cast<const Vec<f16_t, 8> *>(z + (int64_t)m * ld + n);
-    Vec<T, 8> out;
-#pragma unroll
-    for (int e = 0; e < 8; e++) out.v[e] = n + e < N ? (T)((float)g[e] * slope16(act, (float)zz.v[e])) : (T)0.f;
-    *reinterpret_cast<Vec<T, 8> *>(dz + (int64_t)m * ld + n) = out;
+    const uint32_t w = (uint32_t)(i % words);
+    const uint4 g = load_word(dy + (int64_t)m * lddy + w * 8, (int)N - (int)w * 8);       // (zero past N)
+    uint4 z = make_uint4(0, 0, 0, 0);
+    if (keeps_bits(act)) z.x = (uint8_t)kept[m * pitch + w];
+    else z = *reinterpret_cast<const uint4 *>(kept + m * pitch + w * 16);
+    *reinterpret_cast<uint4 *>(dz + (int64_t)m * ld + w * 8) = dz_word<T>(act, g, z);
   }
 }
 
@@ -676,18 +991,24 @@ __global__ void __launch_bounds__(256) transpose_kernel(const T *W, int64_t ldw,
     if (k0 + r + i < K && n0 + c < ld) out[(int64_t)(k0 + r + i) * ld + n0 + c] = tile[c][r + i];
 }
 
-inline uint64_t up(uint64_t v, uint64_t m) { return (v + m - 1) / m * m; }
+// the tall, narrow form: both widths up to 256 in whole words, and rows for a few 64-row tiles per CU
+bool narrow_shape(uint32_t M, uint32_t N, uint32_t K) { return N <= 256 && K <= 256 && N % 8 == 0 && K % 8 == 0 && M >= 16384; }
 
 struct BwdPlan {
-  uint32_t slices, per;
+  uint32_t slices, per;                      // of dz^T x
+  bool narrow;
   uint64_t dz, wt, part, part_b, total;      // byte offsets in the scratch
 };
 
-BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K) {
+#ifndef TN_NARROW_SLICES
+#define TN_NARROW_SLICES 256
+#endif
+BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   BwdPlan p;
+  p.narrow = narrow;
   const uint32_t tiles = ((N + BN - 1) / BN) * ((K + BM - 1) / BM);
   // row slices of dz^T x: one workgroup per CU, at least four stages each
-  uint32_t s = 256 / tiles;
+  uint32_t s = narrow ? TN_NARROW_SLICES : 256 / tiles;
   const uint32_t most = (M + 4 * BK - 1) / (4 * BK);
   s = s < 1 ? 1 : s;
   s = s > most ? most : s;
@@ -697,7 +1018,7 @@ BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K) {
   uint64_t at = 0;
   p.dz = at; at += act ? up((uint64_t)M * up(N, 8) * 2, 256) : 0;
   p.wt = at; at += up((uint64_t)K * up(N, 8) * 2, 256);
-  p.part = at; at += p.slices > 1 ? up((uint64_t)p.slices * N * K * 4, 256) : 0;
+  p.part = at; at += p.slices > 1 || narrow ? up((uint64_t)p.slices * N * K * 4, 256) : 0;
   p.part_b = at; at += up((uint64_t)p.slices * N * 4, 256);
   p.total = at;
   return p;
@@ -714,9 +1035,47 @@ void nt_tiles(GemmArgs a, bool direct, hipStream_t st) {
   else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), g, b, 0, st, a);
 }
 
+#ifndef NARROW_RS
+#define NARROW_RS 6
+#endif
+template <typename T, int SIDE>
+void narrow_launch(const NarrowArgs &n, hipStream_t st) {
+  const uint32_t tiles = (n.g.M + 31) / 32;
+  // (places of the ring by what LDS holds: 96 to 112 KB on their way on a CU)
+#define SHD_NARROW(NWC, KS, RS, PERCU)                                                                                                  \
+  hipLaunchKernelGGL((narrow_kernel<T, NWC, KS, RS, SIDE>), dim3(tiles < 256 * PERCU ? tiles : 256 * PERCU), dim3((NWC + 4) * 64), 0, st, n)
+  if (n.g.N <= 128) {
+    if (n.g.K <= 128) SHD_NARROW(4, 8, 4, 2);
+    else SHD_NARROW(4, 16, 4, 1);
+  } else {
+    if (n.g.K <= 128) SHD_NARROW(8, 8, 5, 1);
+    else SHD_NARROW(8, 16, (SIDE == 1 || SIDE == 2 ? 4 : NARROW_RS), 1);
+  }
+#undef SHD_NARROW
+}
+
+template <typename T, bool BITS>
+void tn_narrow_launch(const TnNarrowArgs &n, hipStream_t st) {
+  const dim3 g(n.t.slices);
+  if (n.t.N <= 128) {
+    if (n.t.K <= 128) hipLaunchKernelGGL((tn_narrow_kernel<T, 1, 2, 4, BITS>), g, dim3(128), 0, st, n);
+    else hipLaunchKernelGGL((tn_narrow_kernel<T, 1, 4, 4, BITS>), g, dim3(256), 0, st, n);
+  } else {
+    if (n.t.K <= 128) hipLaunchKernelGGL((tn_narrow_kernel<T, 2, 2, 4, BITS>), g, dim3(256), 0, st, n);
+    else hipLaunchKernelGGL((tn_narrow_kernel<T, 2, 4, 4, BITS>), g, dim3(512), 0, st, n);
+  }
+}
+
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);
+  if (direct && narrow_shape(a.M, a.N, a.K) && rows_of_words(a.res, a.ldr, a.N, SL_BF16)) {
+    NarrowArgs n = {};
+    n.g = a;
+    if (a.res) narrow_launch<T, 1>(n, st);
+    else narrow_launch<T, 0>(n, st);
+    return;
+  }
   const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
   // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches are rare and take the other)
   if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22)) {
@@ -759,69 +1118,94 @@ int check_sizes(const char *who, int dtype, int act, uint32_t M, uint32_t N, uin
 
 extern "C" int sl_linear16_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, int bias_f32,
                                const void *d_res, int64_t ldr, uint32_t M, uint32_t N, uint32_t K, int act, void *d_y, int64_t ldy,
-                               void *d_z, int64_t ldz, void *stream) {
+                               void *d_kept, void *stream) {
   if (const int rc = check_sizes("sl_linear16_fwd", dtype, act, M, N, K)) return rc;
   if (M == 0) return SG_OK;
   if (!d_x || !d_w || !d_y || ldx < (int64_t)K || ldw < (int64_t)K || ldy < (int64_t)N || (d_res && ldr < (int64_t)N) ||
-      (d_z && (ldz < (int64_t)up(N, 8) || ldz % 8 || (reinterpret_cast<uintptr_t>(d_z) & 15))))
+      (d_kept && (reinterpret_cast<uintptr_t>(d_kept) & 15)))
     return set_error(SG_ERR_INVALID, "sl_linear16_fwd: operands");
   hipStream_t st = (hipStream_t)stream;
   GemmArgs a = {};
   a.A = d_x; a.lda = ldx; a.B = d_w; a.ldb = ldw; a.M = M; a.N = N; a.K = K; a.bias = d_bias; a.bias_f32 = bias_f32; a.res = d_res; a.ldr = ldr;
-  a.C = d_y; a.ldc = ldy; a.z = static_cast<f16_t *>(d_z); a.ldz = ldz; a.act = act;
+  a.C = d_y; a.ldc = ldy; a.kept = act ? static_cast<char *>(d_kept) : nullptr; a.act = act;
   SHD_PROF_FMT(2.0 * ((double)M * K + (double)N * K + (double)M * N * (d_res ? 2 : 1)), 2.0 * M * N * K, st, "linear16_fwd_N%u_K%u", N, K);
   SHD_DISPATCH_16(dtype, nt_launch<T>(a, st));
   SHD_HIP(hipGetLastError());
   return SG_OK;
 }
 
-extern "C" size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K) { return plan_bwd(act, M, N, K).total; }
+extern "C" size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N) {
+  return act > 0 && act < kActs ? (size_t)M * kept_pitch(act, N) : 0;
+}
+
+extern "C" size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K) {
+  const uint64_t a = plan_bwd(act, M, N, K, false).total, b = narrow_shape(M, N, K) ? plan_bwd(act, M, N, K, true).total : 0;
+  return a > b ? a : b;
+}
 
 extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy,
-                               const void *d_z, int64_t ldz, uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw,
+                               const void *d_kept, uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw,
                                int64_t lddw, void *d_db, int db_f32, void *d_scratch, void *stream) {
   if (const int rc = check_sizes("sl_linear16_bwd", dtype, act, M, N, K)) return rc;
   const bool want_w = d_dw || d_db;
-  if (!d_scratch || (M && (!d_dy || lddy < (int64_t)N || (act && (!d_z || ldz != (int64_t)up(N, 8) || (reinterpret_cast<uintptr_t>(d_z) & 15))) || (d_dx && (!d_w || ldw < (int64_t)K || lddx < (int64_t)K)) ||
-                           (want_w && (!d_x || ldx < (int64_t)K)))) ||
-      (d_dw && lddw < (int64_t)K))
+  if (!d_scratch || (reinterpret_cast<uintptr_t>(d_scratch) & 15) || (d_dw && lddw < (int64_t)K) ||
+      (M && (!d_dy || lddy < (int64_t)N || (act && (!d_kept || (reinterpret_cast<uintptr_t>(d_kept) & 15))) ||
+             (d_dx && (!d_w || ldw < (int64_t)K || lddx < (int64_t)K)) || (want_w && (!d_x || ldx < (int64_t)K)))))
     return set_error(SG_ERR_INVALID, "sl_linear16_bwd: operands");
   if (d_db && !d_dw) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: db comes with dW");
   hipStream_t st = (hipStream_t)stream;
-  const BwdPlan p = plan_bwd(act, M, N, K);
+  const bool dy_words = rows_of_words(d_dy, lddy, N, SL_BF16), x_words = rows_of_words(d_x, ldx, K, SL_BF16), shape = narrow_shape(M, N, K);
+  const bool narrow_dx = d_dx && shape && dy_words, narrow_dw = want_w && shape && x_words && (act || dy_words);
+  const bool bits_dw = narrow_dw && keeps_bits(act) && dy_words;       // (dz^T x masks dy itself)
+  const BwdPlan p = plan_bwd(act, M, N, K, narrow_dw);
   char *ws = static_cast<char *>(d_scratch);
-  const void *dz = d_dy;
-  int64_t lddz = lddy;
-  if (act && M) {
-    lddz = (int64_t)up(N, 8);
-    dz = ws + p.dz;
-    const uint64_t need = ((uint64_t)M * (lddz / 8) + 255) / 256;
+  const bool need_dz = act && M && ((d_dx && !narrow_dx) || (want_w && !bits_dw));
+  const int64_t ldp = (int64_t)up(N, 8);
+  const void *dz = need_dz ? ws + p.dz : d_dy;
+  const int64_t lddz = need_dz ? ldp : lddy;
+  const double bytes_dx = 2.0 * ((double)M * K + (double)N * K + (double)M * N);
+  if (need_dz && !narrow_dx) {
+    const uint64_t need = ((uint64_t)M * (ldp / 8) + 255) / 256;
     const dim3 g((uint32_t)(need < 8192 ? need : 8192)), b(256);
-    SHD_PROF_FMT(6.0 * M * N, 0, st, "linear16_dz_N%u", N);
-    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((dz_kernel<T>), g, b, 0, st, (const T *)d_dy, lddy, (const f16_t *)d_z, (T *)(ws + p.dz), lddz, M, N, act));
+    SHD_PROF_FMT(4.0 * M * N + (double)M * kept_pitch(act, N), 0, st, "linear16_dz_N%u", N);
+    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((dz_kernel<T>), g, b, 0, st, (const T *)d_dy, lddy, (const char *)d_kept, (T *)(ws + p.dz), ldp, M, N, act));
     SHD_HIP(hipGetLastError());
   }
-  if (d_dx && M) {
-    const int64_t ldt = (int64_t)up(N, 8);
+  if (narrow_dx) {
+    NarrowArgs n = {};
+    n.g.A = d_dy; n.g.lda = lddy; n.g.B = d_w; n.g.ldb = ldw; n.g.M = M; n.g.N = K; n.g.K = N; n.g.C = d_dx; n.g.ldc = lddx;
+    n.b_cols = 1; n.kept = static_cast<const char *>(d_kept); n.kept_act = act; n.dz = need_dz ? ws + p.dz : nullptr; n.lddz = ldp;
+    SHD_PROF_FMT(bytes_dx + (act ? (double)M * kept_pitch(act, N) : 0), 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, if (!act) narrow_launch<T, 0>(n, st);
+                    else if (keeps_bits(act)) narrow_launch<T, 3>(n, st);
+                    else narrow_launch<T, 2>(n, st));
+    SHD_HIP(hipGetLastError());
+  } else if (d_dx && M) {
     GemmArgs a = {};
-    a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldt; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
-    a.K = act ? (uint32_t)ldt : N;           // (dz of an activation has zero pad columns, as W^T has: whole words)
-    SHD_PROF_FMT(2.0 * ((double)M * K + (double)N * K + (double)M * N), 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((transpose_kernel<T>), dim3((K + 31) / 32, (uint32_t)((ldt + 31) / 32)), dim3(256), 0, st, (const T *)d_w, ldw, N, K,
-                                              (T *)(ws + p.wt), ldt);
+    a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldp; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
+    a.K = act ? (uint32_t)ldp : N;           // (dz of an activation has zero pad columns, as W^T has: whole words)
+    SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((transpose_kernel<T>), dim3((K + 31) / 32, (uint32_t)((ldp + 31) / 32)), dim3(256), 0, st, (const T *)d_w, ldw, N, K,
+                                              (T *)(ws + p.wt), ldp);
                     nt_launch<T>(a, st));
     SHD_HIP(hipGetLastError());
   }
   if (want_w) {
-    TnArgs a = {};
-    a.A = dz; a.lda = lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + BN - 1) / BN; a.tiles_k = (K + BM - 1) / BM;
-    a.slices = p.slices; a.per = p.per; a.part = p.slices > 1 ? reinterpret_cast<float *>(ws + p.part) : nullptr;
-    a.part_b = d_db ? reinterpret_cast<float *>(ws + p.part_b) : nullptr; a.C = d_dw; a.ldc = lddw;
-    const bool da = act || rows_of_words(dz, lddz, N, SL_BF16), db = rows_of_words(d_x, ldx, K, SL_BF16);
-    SHD_PROF_FMT(2.0 * ((double)M * K + (double)N * K + (double)M * N), 2.0 * M * N * K, st, "linear16_dw_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, tn_launch<T>(a, da, db, st);
-                    if (p.slices > 1) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)(((uint64_t)N * K + 255) / 256)), dim3(256), 0, st, a.part, p.slices, N, K, (T *)d_dw, lddw);
-                    if (d_db) hipLaunchKernelGGL((bias_join_kernel<T>), dim3((N + 255) / 256), dim3(256), 0, st, a.part_b, p.slices, N, d_db, db_f32));
+    TnNarrowArgs n = {};
+    TnArgs &a = n.t;
+    a.A = bits_dw ? d_dy : dz; a.lda = bits_dw ? lddy : lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + BN - 1) / BN;
+    a.tiles_k = (K + BM - 1) / BM; a.slices = p.slices; a.per = p.per; a.C = d_dw; a.ldc = lddw;
+    a.part = p.slices > 1 || narrow_dw ? reinterpret_cast<float *>(ws + p.part) : nullptr;
+    a.part_b = d_db ? reinterpret_cast<float *>(ws + p.part_b) : nullptr;
+    n.kept = static_cast<const char *>(d_kept); n.kept_act = act;
+    const bool da = act || dy_words;
+    const uint64_t joined = (a.part ? (uint64_t)N * K : 0) + (d_db ? N : 0);
+    SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dw_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, da, x_words, st);
+                    else if (bits_dw) tn_narrow_launch<T, true>(n, st);
+                    else tn_narrow_launch<T, false>(n, st);
+                    if (joined) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)((joined + 255) / 256)), dim3(256), 0, st, a.part, a.part_b, p.slices, N, K,
+                                                   (T *)d_dw, lddw, d_db, db_f32));
     SHD_HIP(hipGetLastError());
   }
   return SG_OK;

@@ -209,33 +209,34 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor, None] = No
 
 # ---------------------------------------------------------------- the 16-bit Linear
 
-def _lin_fwd(x, W, b, residual, act, want_z):
+def _lin_fwd(x, W, b, residual, act, keep):
     x2, r2, W = _rows(x), _rows(residual), _rows(W)
     M, K = x2.shape
     N = W.shape[0]
     y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-    z = torch.empty(M, (N + 7) // 8 * 8, dtype=torch.float16, device=x.device) if want_z else None
+    lib = _lib.load()
+    kept = torch.empty(max(16, int(lib.sl_linear16_kept_bytes(act, M, N))), dtype=torch.uint8, device=x.device) if keep else None
     if M:
         with _on(x.device):
-            check(_lib.load().sl_linear16_fwd(_DT[x.dtype], x2.data_ptr(), x2.stride(0), W.data_ptr(), W.stride(0), _ptr(b),
-                                              int(b is not None and b.dtype == torch.float32), _ptr(r2), _ld(r2), M, N, K, act,
-                                              y.data_ptr(), N, _ptr(z), _ld(z), _stream(x)))
-    return y, z
+            check(lib.sl_linear16_fwd(_DT[x.dtype], x2.data_ptr(), x2.stride(0), W.data_ptr(), W.stride(0), _ptr(b),
+                                      int(b is not None and b.dtype == torch.float32), _ptr(r2), _ld(r2), M, N, K, act,
+                                      y.data_ptr(), N, _ptr(kept), _stream(x)))
+    return y, kept
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b, residual, act):
-        y, z = _lin_fwd(x, W, b, residual, act, act != 0)
+        y, kept = _lin_fwd(x, W, b, residual, act, act != 0)
         ctx.act = act
         ctx.bias = None if b is None else b.dtype
-        ctx.save_for_backward(x, W, z)
+        ctx.save_for_backward(x, W, kept)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, W, z = ctx.saved_tensors
+        x, W, kept = ctx.saved_tensors
         x2, w2, dy2 = _rows(x), _rows(W), _rows(dy)
         M, K = x2.shape
         N = w2.shape[0]
@@ -251,7 +252,7 @@ class _LinearAct(torch.autograd.Function):
         ws = torch.empty(max(16, int(lib.sl_linear16_bwd_scratch_bytes(ctx.act, M, N, K))), dtype=torch.uint8, device=dev)
         with _on(dev):
             check(lib.sl_linear16_bwd(_DT[x.dtype], x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), dy2.data_ptr(), dy2.stride(0),
-                                      _ptr(z), _ld(z), M, N, K, ctx.act, _ptr(dx), K, _ptr(dW), K, _ptr(db), int(ctx.bias == torch.float32),
+                                      _ptr(kept), M, N, K, ctx.act, _ptr(dx), K, _ptr(dW), K, _ptr(db), int(ctx.bias == torch.float32),
                                       ws.data_ptr(), _stream(x)))
         return dx, (dW if need[1] else None), db, dres, None
 
@@ -262,8 +263,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     bias ``[N]`` in that type or fp32; products and the epilogue in fp32, one rounding at the end.  ``act``: a key of
     ``LINEAR_ACT_CODE``.  fp32 operands go through ``ops.linear`` / ``ops.linear_act_norm``.
 
-    For the backward pass the pre-activation is kept in fp16 and ``dz = dy act'(z)`` is rounded to the operands' type (the matrix cores
-    take 16-bit operands); an identity keeps nothing and rounds nothing."""
+    For the backward pass one bit of every pre-activation is kept (relu, leakyrelu) or its fp16 value (the others), and
+    ``dz = dy act'(z)`` is rounded to the operands' type (the matrix cores take 16-bit operands); an identity keeps and rounds nothing."""
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"linear_act: {x.dtype} (bfloat16 or float16; fp32 products are ops.linear / ops.linear_act_norm)")
     _float_rows("linear_act", x)

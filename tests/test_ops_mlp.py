@@ -65,7 +65,7 @@ def test_python_entries_refuse(call, error):
 
 
 _BUF = (C.c_char * 4096)()
-P = C.addressof(_BUF)          # a host address: the calls below return before any kernel could see it
+P = (C.addressof(_BUF) + 255) // 256 * 256          # a host address: the calls below return before any kernel could see it
 
 
 @pytest.mark.parametrize("name,args", [
@@ -85,15 +85,15 @@ P = C.addressof(_BUF)          # a host address: the calls below return before a
     ("sl_dropout", (1, P, 4, None, 0, 1, 8, 0.5, 1, None, P, 8, None)),
     ("sl_dropout", (1, P, 8, P, 4, 1, 8, 0.5, 1, None, P, 8, None)),
     ("sl_dropout", (1, P, 8, None, 0, 1, 8, 0.5, 1, None, None, 8, None)),
-    ("sl_linear16_fwd", (0, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 0, P, 8, None, 0, None)),     # fp32
-    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 7, P, 8, None, 0, None)),     # activation
-    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 0, 8, 0, P, 8, None, 0, None)),     # N = 0
-    ("sl_linear16_fwd", (1, P, 4, P, 8, None, 0, None, 0, 1, 8, 8, 0, P, 8, None, 0, None)),     # pitch
-    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, P, 4, 1, 8, 8, 0, P, 8, None, 0, None)),        # residual pitch
-    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 1, P, 8, P, 12, None)),       # z pitch
-    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 0, 1, 8, 8, 1, P, 8, None, 0, None, 0, P, None)),    # an activation without z
-    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 0, 1, 8, 8, 0, P, 8, None, 0, P, 0, P, None)),       # db without dW
-    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 0, 1, 8, 8, 0, P, 8, None, 0, None, 0, None, None)),  # no scratch
+    ("sl_linear16_fwd", (0, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 0, P, 8, None, None)),     # fp32
+    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 7, P, 8, None, None)),     # activation
+    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 0, 8, 0, P, 8, None, None)),     # N = 0
+    ("sl_linear16_fwd", (1, P, 4, P, 8, None, 0, None, 0, 1, 8, 8, 0, P, 8, None, None)),     # pitch
+    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, P, 4, 1, 8, 8, 0, P, 8, None, None)),        # residual pitch
+    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, 1, 8, 8, 1, P, 8, P + 8, None)),       # alignment of what is kept
+    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 1, 8, 8, 1, P, 8, None, 0, None, 0, P, None)),    # an activation without what it kept
+    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 1, 8, 8, 0, P, 8, None, 0, P, 0, P, None)),       # db without dW
+    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 8, None, 1, 8, 8, 0, P, 8, None, 0, None, 0, None, None)),  # no scratch
     ("sl_label_logprobs_fwd", (5, P, 8, P, 1, 1, 8, 0, P, P, P, None, None, None, None)),
     ("sl_label_logprobs_fwd", (1, P, 8, P, 1, 1, 8, 9, P, P, P, P, P, None, None)),              # k > C
     ("sl_label_logprobs_fwd", (1, P, 100, P, 1, 1, 100, 65, P, P, P, P, P, None, None)),         # k > 64
@@ -117,3 +117,4 @@ def test_sizes_of_scratch():
     assert lib.sl_label_logprobs_scratch_bytes(0, 1000, 47, 5) == 0          # rows in registers
     assert lib.sl_label_logprobs_scratch_bytes(1, 1, 131072, 10) > 0         # one row: split
     assert lib.sl_linear16_bwd_scratch_bytes(1, 0, 8, 8) > 0
+    assert lib.sl_linear16_kept_bytes(0, 10, 64) == 0 and lib.sl_linear16_kept_bytes(1, 10, 129) == 320 and lib.sl_linear16_kept_bytes(5, 10, 129) == 10 * 136 * 2

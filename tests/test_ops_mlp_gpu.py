@@ -25,12 +25,13 @@ def _half(dtype):
 
 
 def _assert_within(got, want, tol, what):
-    """|got - want| <= half a step of got's type + tol, element by element; NaN and infinities agree."""
+    """|got - want| <= half a step of got's type + tol, element by element; NaN and infinities agree.  What is rounded is the value v
+    with |v - want| <= tol, so the half step is one of |v| <= |want| + tol: |got - want| <= tol + eps / 2 (|want| + tol)."""
     got64, want = got.detach().double(), want.detach().double()
     assert got64.shape == want.shape, what
     same = (got64 == want) | (got64.isnan() & want.isnan())
     tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps      # (a subnormal result: half its step)
-    bad = ~same & ~((got64 - want).abs() <= _half(got.dtype) * want.abs() * (1 + 1e-6) + tiny + tol)
+    bad = ~same & ~((got64 - want).abs() <= _half(got.dtype) * (want.abs() + tol) * (1 + 1e-6) + tiny + tol)
     if bad.any():
         at = bad.nonzero()[0].tolist()
         t = tol.expand(want.shape)[tuple(at)].item() if isinstance(tol, torch.Tensor) else tol
@@ -315,6 +316,33 @@ def test_linear_act(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["I", "relu", "leakyrelu", "gelu"])
+@pytest.mark.parametrize("M,N,K", [(16384, 256, 256), (20001, 256, 128), (16400, 128, 256), (33333, 64, 96), (16447, 40, 128), (17000, 200, 256), (16385, 248, 136), (16384, 8, 8)])
+def test_linear_act_tall_and_narrow(dtype, act, M, N, K):
+    """The form with the weight in registers, its gradients with dy masked (or dz formed) in the tile."""
+    g = _gen(M + N + K)
+    x, W = _randn(g, M, K, dtype=dtype), _randn(g, N, K, dtype=dtype, scale=K ** -0.5)
+    _lin_check(x, W, _randn(g, N), act, _randn(g, M, N, dtype=dtype), _randn(g, M, N, dtype=dtype))
+
+
+@pytest.mark.parametrize("act", ["I", "relu", "tanh"])
+def test_linear_act_tall_and_narrow_in_parts(act):
+    """Single gradients, pitched operands and rows that are no whole words: the forms mix."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(71)
+    M, N, K = 16500, 96, 104
+    x, W, b, dy = _randn(g, M, K, dtype=BF16), _randn(g, N, K, dtype=BF16, scale=0.1), _randn(g, N), _randn(g, M, N, dtype=BF16)
+    full = [t.clone().requires_grad_(True) for t in (x, W, b)]
+    full = torch.autograd.grad(ops_mlp.linear_act(*full, act=act), full, dy)
+    for i in range(3):
+        ins = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, W, b))]
+        got, = torch.autograd.grad(ops_mlp.linear_act(*ins, act=act), (ins[i],), dy)
+        assert torch.equal(got, full[i]), i
+    for xv, dv in ((_pitched(x, 112), _pitched(dy, 104)), (_pitched(x, 105), dy), (x, _pitched(dy, 97)), (_pitched(x, 104, 1), _pitched(dy, 96, 3))):
+        _lin_check(xv, W, b, act, None, dv)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("act", ["I", "relu", "elu", "tanh", "leakyrelu", "gelu", "silu"])
 def test_linear_act_activations(dtype, act):
     g = _gen(31)
@@ -576,15 +604,15 @@ def test_rows_behind_the_last_stay_as_they_were():
         stat = torch.full((4, n + 5), 5.0, device=DEV)
         lab = torch.zeros(n, dtype=torch.int64, device=DEV)
         ws = torch.empty(1 << 24, dtype=torch.uint8, device=DEV)
-        z = torch.zeros(n, (F + 7) // 8 * 8, dtype=F16, device=DEV)
+        kept = torch.zeros(n * 1024, dtype=torch.uint8, device=DEV)
         for off in (0, 1):
             calls = {
                 "ln": lambda y: lib.sl_layer_norm_fwd(1, 0, x.data_ptr(), F, None, None, n, F, 1e-5, y, pitch, None, st),
                 "ln_bwd": lambda y: lib.sl_layer_norm_bwd(1, 0, x.data_ptr(), F, r.data_ptr(), F, None, stat.data_ptr(), n, F, y, pitch, None, None, None, st),
                 "drop": lambda y: lib.sl_dropout(1, x.data_ptr(), F, r.data_ptr(), F, n, F, 0.5, 3, None, y, pitch, st),
-                "lin": lambda y: lib.sl_linear16_fwd(1, x.data_ptr(), F, W.data_ptr(), F, None, 0, r.data_ptr(), F, n, F, F, 1, y, pitch, z.data_ptr(), z.stride(0), st),
-                "lin_dx": lambda y: lib.sl_linear16_bwd(1, x.data_ptr(), F, W.data_ptr(), F, r.data_ptr(), F, z.data_ptr(), z.stride(0), n, F, F, 1, y, pitch, None, 0, None, 0, ws.data_ptr(), st),
-                "lin_dw": lambda y: lib.sl_linear16_bwd(1, x[:, :37].contiguous().data_ptr() if F > 37 else 0, 37, W.data_ptr(), F, r.data_ptr(), F, None, 0, n, 37, 37, 0, None, 0, y, pitch, None, 0, ws.data_ptr(), st),
+                "lin": lambda y: lib.sl_linear16_fwd(1, x.data_ptr(), F, W.data_ptr(), F, None, 0, r.data_ptr(), F, n, F, F, 1, y, pitch, kept.data_ptr(), st),
+                "lin_dx": lambda y: lib.sl_linear16_bwd(1, x.data_ptr(), F, W.data_ptr(), F, r.data_ptr(), F, kept.data_ptr(), n, F, F, 1, y, pitch, None, 0, None, 0, ws.data_ptr(), st),
+                "lin_dw": lambda y: lib.sl_linear16_bwd(1, x[:, :37].contiguous().data_ptr() if F > 37 else 0, 37, W.data_ptr(), F, r.data_ptr(), F, None, n, 37, 37, 0, None, 0, y, pitch, None, 0, ws.data_ptr(), st),
                 "lp_bwd": lambda y: lib.sl_label_logprobs_bwd(1, x.data_ptr(), F, lab.data_ptr(), 1, n, F, 0, stat[0].data_ptr(), stat[1].data_ptr(), None, stat[2].data_ptr(), None, None, y, pitch, st),
             }
             for name, call in calls.items():
