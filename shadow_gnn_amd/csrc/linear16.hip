@@ -142,13 +142,14 @@ __device__ __forceinline__ void lds_dma16(const void *src, void *dst) {
 }
 
 // The same transfer in inline assembly, for kernels that keep several stages in flight: the compiler would wait for all of them before
-// every LDS read.  It has no result register; the kernel counts the transfers itself (wait_vm).  m0 needs one wait state before its use.
+// every LDS read.  It has no result register; the kernel counts the transfers itself (wait_vm).  m0 (a register
+// the compiler writes in front of each use of its own) needs one wait state before its use.
 // First form: an address per lane; second: a uniform base and an offset per lane, nothing to compute from stage to stage.
 __device__ __forceinline__ void lds_dma16_async(const void *src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
 }
 __device__ __forceinline__ void lds_dma16_async(const void *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
 // One barrier per tile: the tile is whole, and the one before it has been read.
 //   SIDE 1: the residual's rows.
 //   SIDE 2, 3 (dx = dz W; A is dy): kept fp16 values / kept bits.  The tile becomes dz = dy act'(z) in place, each wavefront a share
-//   of it, and is stored for dz^T x if asked for; a second barrier then.
+//   of it, while the tile before it is multiplied, and is stored for dz^T x if asked for.
 // Bits kept by the forward pass are gathered in LDS and leave a tile later as whole words (as bytes they cost 25 us of 140).
 struct NarrowArgs {
   GemmArgs g;
@@ -600,12 +601,15 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
     for (int s = 0; s < RS - 1; s++)
       if (next < tiles) { send(next, slot); next += gridDim.x; slot++; }
     uint32_t left = slot;                    // tiles sent and not yet awaited
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    auto await = [&]() {                     // the oldest tile sent is whole
       if (left == RS - 1) wait_vm<(RS - 2) * PER>();
       else wait_vm<0>();
       left--;
+    };
+    if (SIDE >= 2) { await(); __syncthreads(); }
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      if (SIDE < 2 || tile + gridDim.x < tiles) await();
       __syncthreads();
-      if (SIDE >= 2) __syncthreads();
       if (next < tiles) { send(next, slot); next += gridDim.x; left++; slot = slot + 1 == RS ? 0 : slot + 1; }
     }
     if (bits_out) __syncthreads();
@@ -615,20 +619,32 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
   const uint32_t n0 = wave * 32;
   v8 fb[KS];                                 // B's rows n0 + (lane & 31): the step's eight elements of this lane
   {
+    // (loads without conditions, so that all are on their way together; K is a multiple of eight: a lane's eight exist or not)
     const uint32_t row = min(n0 + (lane & 31), a.N - 1);
+    if (n.b_cols) {
 #pragma unroll
-    for (int q = 0; q < KS; q++) {
-      const uint32_t k = q * 16 + (lane >> 5) * 8;
-      if (n.b_cols) {
+      for (int q = 0; q < KS; q++) {
+        const uint32_t k = q * 16 + (lane >> 5) * 8;
+        const T *p = static_cast<const T *>(a.B) + (int64_t)(k < a.K ? k : 0) * a.ldb + row;
         T e[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = k + j < a.K ? static_cast<const T *>(a.B)[(int64_t)(k + j) * a.ldb + row] : (T)0.f;
+        for (int j = 0; j < 8; j++) e[j] = p[j * a.ldb];
         __builtin_memcpy(&fb[q], e, 16);
-      } else {
-        const uint4 w = load_word(static_cast<const T *>(a.B) + (int64_t)row * a.ldb + k, (int)a.K - (int)k);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < KS; q++) {
+        const uint32_t k = q * 16 + (lane >> 5) * 8;
+        const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.B) + (int64_t)row * a.ldb + (k < a.K ? k : 0));
         __builtin_memcpy(&fb[q], &w, 16);
       }
     }
+#pragma unroll
+    for (int q = 0; q < KS; q++)
+      if (q * 16 + (lane >> 5) * 8 >= a.K) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        __builtin_memcpy(&fb[q], &zero, 16);
+      }
   }
   float *mine = reinterpret_cast<float *>(lds + RS * kPlace) + wave * 512;             // 16 rows of 32 columns
   uint8_t *bits = reinterpret_cast<uint8_t *>(lds + RS * kPlace + NWC * 2048);         // two tiles of R rows, 32 bytes each
@@ -644,6 +660,23 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
   if (bits_out) {                            // (columns past N: no bits)
     for (uint32_t w = threadIdx.x; w < 2 * R * 8; w += NWC * 64) reinterpret_cast<uint32_t *>(bits)[w] = 0;
   }
+  auto form_dz = [&](char *place, uint32_t row0) {
+#pragma unroll
+    for (int i = 0; i < R * W / (NWC * 64); i++) {
+      const uint32_t w = i * NWC * 64 + threadIdx.x, r = w / W, c = w % W;
+      uint4 *p = reinterpret_cast<uint4 *>(place + (r * W + swz_row<W>(r, c)) * 16);
+      uint4 z = make_uint4(0, 0, 0, 0);
+      if constexpr (SIDE == 2) z = *reinterpret_cast<const uint4 *>(place + kA + (r * W + swz_row<W>(r, c)) * 16);
+      else if (c * 8 < a.K) z.x = *reinterpret_cast<const uint8_t *>(place + kA + r * (kept_pitch(1, a.K)) + c);
+      const uint4 d = dz_word<T>(n.kept_act, *p, z);
+      *p = d;
+      if (n.dz && row0 + r < a.M && c * 8 < a.K) *reinterpret_cast<uint4 *>(static_cast<T *>(n.dz) + (int64_t)(row0 + r) * n.lddz + c * 8) = d;
+    }
+  };
+  if constexpr (SIDE >= 2) {
+    __syncthreads();
+    form_dz(lds, blockIdx.x * R);
+  }
   uint32_t at = 0, turn = 0;
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
     char *cur = lds + at * kPlace;
@@ -652,25 +685,27 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
     const uint32_t m0 = tile * R;
     if (bits_out && tile != blockIdx.x) flush_bits(tile - gridDim.x, turn ^ 1);
     if constexpr (SIDE >= 2) {
-#pragma unroll
-      for (int i = 0; i < R * W / (NWC * 64); i++) {
-        const uint32_t w = i * NWC * 64 + threadIdx.x, r = w / W, c = w % W;
-        uint4 *p = reinterpret_cast<uint4 *>(cur + (r * W + swz_row<W>(r, c)) * 16);
-        uint4 z = make_uint4(0, 0, 0, 0);
-        if constexpr (SIDE == 2) z = *reinterpret_cast<const uint4 *>(cur + kA + (r * W + swz_row<W>(r, c)) * 16);
-        else if (c * 8 < a.K) z.x = *reinterpret_cast<const uint8_t *>(cur + kA + r * (kept_pitch(1, a.K)) + c);
-        const uint4 d = dz_word<T>(n.kept_act, *p, z);
-        *p = d;
-        if (n.dz && m0 + r < a.M && c * 8 < a.K) *reinterpret_cast<uint4 *>(static_cast<T *>(n.dz) + (int64_t)(m0 + r) * n.lddz + c * 8) = d;
-      }
-      __syncthreads();
+      if (tile + gridDim.x < tiles) form_dz(lds + at * kPlace, m0 + gridDim.x * R);
     }
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    // (operands are read eight steps ahead, four at a time: left to itself the compiler reads one ahead and waits for LDS at every product)
     const uint32_t ra = lane & 31;
+    v8 fa[8];
 #pragma unroll
-    for (int q = 0; q < KS; q++) acc = mma(fb[q], *reinterpret_cast<const v8 *>(cur + (ra * W + swz_row<W>(ra, q * 2 + (lane >> 5))) * 16), acc);
+    for (int q = 0; q < 8; q++) fa[q] = *reinterpret_cast<const v8 *>(cur + (ra * W + swz_row<W>(ra, q * 2 + (lane >> 5))) * 16);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < KS / 4; g++) {
+#pragma unroll
+      for (int q = 0; q < 4; q++) acc = mma(fb[g * 4 + q], fa[(g & 1) * 4 + q], acc);
+      if (g + 2 < KS / 4) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) fa[(g & 1) * 4 + q] = *reinterpret_cast<const v8 *>(cur + (ra * W + swz_row<W>(ra, (g * 4 + 8 + q) * 2 + (lane >> 5))) * 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (uint32_t h = 0; h < 2; h++) {       // 16 rows at a time through this wavefront's corner (word w of row r at w ^ ((r >> 1) & 7))
       if (((lane >> 4) & 1) == h) {
@@ -831,6 +866,8 @@ __global__ void __launch_bounds__(kThreads, 2) tn_kernel(TnArgs a) {
 
 // dz^T x of narrow operands (N <= 128 NB, K <= 64 KB): one workgroup holds all of dW -- 128 x 64 per wavefront -- and walks one row
 // slice, 32 rows a stage, both operands read once.  BITS: A is dy and its stage is masked in place by relu's (leakyrelu's) kept bits.
+// (Two workgroups per slice of 128 columns of dz each halve the partial products but read x twice: 120 + 9 instead of 80 + 15 us at
+// 289127 x 256 x 256.)
 // db: dz^T 1 on the same products, the 32-column groups of a 128-column block dealt to the block's KB wavefronts.
 struct TnNarrowArgs {
   TnArgs t;
@@ -1000,15 +1037,12 @@ struct BwdPlan {
   uint64_t dz, wt, part, part_b, total;      // byte offsets in the scratch
 };
 
-#ifndef TN_NARROW_SLICES
-#define TN_NARROW_SLICES 256
-#endif
 BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   BwdPlan p;
   p.narrow = narrow;
   const uint32_t tiles = ((N + BN - 1) / BN) * ((K + BM - 1) / BM);
   // row slices of dz^T x: one workgroup per CU, at least four stages each
-  uint32_t s = narrow ? TN_NARROW_SLICES : 256 / tiles;
+  uint32_t s = narrow ? 256 : 256 / tiles;
   const uint32_t most = (M + 4 * BK - 1) / (4 * BK);
   s = s < 1 ? 1 : s;
   s = s > most ? most : s;
@@ -1035,9 +1069,6 @@ void nt_tiles(GemmArgs a, bool direct, hipStream_t st) {
   else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), g, b, 0, st, a);
 }
 
-#ifndef NARROW_RS
-#define NARROW_RS 6
-#endif
 template <typename T, int SIDE>
 void narrow_launch(const NarrowArgs &n, hipStream_t st) {
   const uint32_t tiles = (n.g.M + 31) / 32;
@@ -1049,7 +1080,7 @@ void narrow_launch(const NarrowArgs &n, hipStream_t st) {
     else SHD_NARROW(4, 16, 4, 1);
   } else {
     if (n.g.K <= 128) SHD_NARROW(8, 8, 5, 1);
-    else SHD_NARROW(8, 16, (SIDE == 1 || SIDE == 2 ? 4 : NARROW_RS), 1);
+    else SHD_NARROW(8, 16, (SIDE == 1 || SIDE == 2 ? 4 : 6), 1);
   }
 #undef SHD_NARROW
 }
