@@ -312,6 +312,25 @@ def load():
     return lib
 
 
+_ops_mlp = None
+
+
+def load_ops_mlp():
+    """The host side of ops_mlp (_ops_mlp.so, csrc/ops_mlp.cpp), linked against libshadow_hip.so beside it."""
+    global _ops_mlp
+    if _ops_mlp is None:
+        load()
+        try:
+            from . import _ops_mlp as mod
+        except ImportError as e:
+            raise ImportError("shadow_gnn_amd/_ops_mlp.so does not load: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                              f"at the repo root ({e})") from e
+        if mod.abi_version() != ABI_VERSION:
+            raise ImportError("shadow_gnn_amd/_ops_mlp.so belongs to another libshadow_hip.so: rebuild it")
+        _ops_mlp = mod
+    return _ops_mlp
+
+
 def check(code):
     if code == SG_OK:
         return
