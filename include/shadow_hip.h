@@ -936,7 +936,7 @@ int sl_gat_bwd_map(const uint32_t *d_indptr, const uint32_t *d_indices, const ui
  * every row, which the backward pass reads.  (The normalisation of shaDow/layers.py:329-338 without its activation.) */
 int sl_layer_norm_fwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, const void *d_scale, const void *d_offset, uint32_t n,
                       uint32_t F, float eps, void *d_y, int64_t ldy, float *d_stats, void *stream);
-/* dx, dscale [F], doffset [F] (each may be NULL); d_partial: sl_layer_norm_partial_floats(n, F) floats, needed for dscale / doffset.
+/* dx, dscale [F], doffset [F] (each may be NULL); d_partial: sl_layer_norm_partial_floats(n, F) floats for dscale / doffset (none: NULL).
  * n == 0 writes zeros there. */
 size_t sl_layer_norm_partial_floats(uint32_t n, uint32_t F);
 int sl_layer_norm_bwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const void *d_scale,

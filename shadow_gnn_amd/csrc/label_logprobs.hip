@@ -37,7 +37,7 @@ struct LpArgs {
   // streaming form: partials of the splits of a row
   uint32_t splits;
   float *part;                                // [n, splits, 4]: M, S, T, -
-  int2 *part_top;                             // [n, splits, k]: key, index
+  int2 *part_top;                             // [n, splits, 4 wavefronts, k]: key, index
 };
 
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }      // NaN wins
@@ -51,12 +51,29 @@ __device__ __forceinline__ float value_of(int32_t key) {
   return key == INT32_MAX ? __int_as_float(0x7FC00000) : __int_as_float(key ^ ((key >> 31) & 0x7FFFFFFF));
 }
 
-// all-reduce over aligned groups of LS lanes with a binary op
-template <int LS, typename Op, typename V>
-__device__ __forceinline__ V group_all(V v, Op op) {
-#pragma unroll
-  for (int off = 1; off < LS; off <<= 1) v = op(v, __shfl_xor(v, off, 64));
+// all-reduce over aligned groups of LS lanes with a commutative, idempotent op, on the DPP network (group_sum's steps; through the LDS
+// crossbar the five alternatives of 289127 rows of 172 alone took 45 us)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+template <int LS, typename Op>
+__device__ __forceinline__ uint32_t group_all(uint32_t v, Op op) {
+  if (LS >= 2) v = op(v, dpp<0xB1>(v));
+  if (LS >= 4) v = op(v, dpp<0x4E>(v));
+  if (LS >= 8) v = op(v, dpp<0x141>(v));
+  if (LS >= 16) v = op(v, dpp<0x140>(v));
+  if (LS >= 32) {
+    const auto sw = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(sw[0], sw[1]);
+  }
+  if (LS >= 64) {
+    const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(sw[0], sw[1]);
+  }
   return v;
+}
+template <int LS>
+__device__ __forceinline__ float group_nan_max(float v) {
+  return __uint_as_float(group_all<LS>(__float_as_uint(v), [](uint32_t p, uint32_t q) { return __float_as_uint(nan_max(__uint_as_float(p), __uint_as_float(q))); }));
 }
 
 // u of a logit (M = -inf: no finite logit, NaN difference -> -1000; a row with +inf or NaN is told by log2 S = NaN)
@@ -102,7 +119,7 @@ __global__ void __launch_bounds__(256) lp_rows_kernel(LpArgs a) {
 #pragma unroll
     for (int j = 0; j < V; j++) m = nan_max(m, v[i][j]);
   }
-  m = group_all<L>(m, nan_max);
+  m = group_nan_max<L>(m);
   float S = 0.f, Tt = 0.f;
 #pragma unroll
   for (int i = 0; i < NC; i++)
@@ -130,7 +147,7 @@ __global__ void __launch_bounds__(256) lp_rows_kernel(LpArgs a) {
     for (int i = 0; i < NC; i++)
 #pragma unroll
       for (int j = 0; j < V; j++) best = max(best, key[i][j]);
-    best = group_all<L>(best, [](int32_t p, int32_t q) { return max(p, q); });
+    best = (int32_t)group_all<L>((uint32_t)best, [](uint32_t p, uint32_t q) { return (uint32_t)max((int32_t)p, (int32_t)q); });
     uint32_t at = 0xFFFFFFFFu;
 #pragma unroll
     for (int i = NC - 1; i >= 0; i--)
@@ -154,13 +171,18 @@ struct Best {
   int32_t key;
   int32_t idx;
   int32_t thr_key, thr_idx;                   // the k-th (uniform)
-  float thr;                                  // its value as a float for the quick test (NaN-safe: !(x < thr))
+  int32_t floor;                              // a key that the k-th reaches, known before the list is full
+  float thr;                                  // max(floor, k-th) as a float for the quick test (NaN-safe: !(x < thr))
 };
 
 __device__ __forceinline__ bool better(int32_t k, int32_t i, int32_t k2, int32_t i2) { return k > k2 || (k == k2 && i < i2); }
 
 __device__ __forceinline__ void best_init(Best &b) {
-  b.key = kNoKey; b.idx = INT32_MAX; b.thr_key = kNoKey; b.thr_idx = INT32_MAX; b.thr = -INFINITY;
+  b.key = kNoKey; b.idx = INT32_MAX; b.thr_key = kNoKey; b.thr_idx = INT32_MAX; b.floor = kNoKey; b.thr = -INFINITY;
+}
+__device__ __forceinline__ void best_quick(Best &b) {
+  const int32_t t = max(b.thr_key, b.floor);
+  b.thr = t == kNoKey ? -INFINITY : value_of(t);
 }
 
 // offer one (key, idx) per lane; every lane of the wavefront calls it
@@ -171,7 +193,7 @@ __device__ __forceinline__ void best_offer(Best &b, int32_t key, int32_t idx, ui
     const int32_t ck = __builtin_amdgcn_readlane(key, src), ci = __builtin_amdgcn_readlane(idx, src);
     const uint32_t lane = lane_id();
     const int at = __popcll(__ballot(better(b.key, b.idx, ck, ci)));            // entries that stay in front
-    const int32_t pk = __shfl_up(b.key, 1, 64), pi = __shfl_up(b.idx, 1, 64);
+    const int32_t pk = (int32_t)dpp<0x138>((uint32_t)b.key), pi = (int32_t)dpp<0x138>((uint32_t)b.idx);        // (wave_shr:1: the lane below)
     b.key = (int)lane < at ? b.key : (int)lane == at ? ck : pk;
     b.idx = (int)lane < at ? b.idx : (int)lane == at ? ci : pi;
     b.thr_key = __builtin_amdgcn_readlane(b.key, (int)k - 1);
@@ -179,7 +201,7 @@ __device__ __forceinline__ void best_offer(Best &b, int32_t key, int32_t idx, ui
     cand &= ~(1ull << src);
     cand &= __ballot(better(key, idx, b.thr_key, b.thr_idx));
   }
-  b.thr = b.thr_key == kNoKey ? -INFINITY : value_of(b.thr_key);
+  best_quick(b);
 }
 
 // joins (M, S, T) of two disjoint parts (M = -inf: one without a finite logit, S = T = 0)
@@ -215,6 +237,33 @@ __device__ __forceinline__ void feed_stats(const float (&v)[W][V], float &M, flo
     }
 }
 
+// A lower bound for the k-th best from one value per lane (the lanes' maxima): the k-th largest of them -- at least k values reach it.
+// A wavefront's first trip uses it, when the list is still empty and nearly everything would be offered: 2048 values then offer some
+// k + 5 instead of k (1 + ln(2048 / k)).  Found by counting, for each lane, the lanes that beat it.
+__device__ __forceinline__ int32_t kth_of_lanes(int32_t key, uint32_t k) {
+  uint32_t above = 0;
+#pragma unroll 8
+  for (int l = 0; l < 64; l++) above += __builtin_amdgcn_readlane(key, l) > key ? 1u : 0u;
+  return (int32_t)group_all<64>((uint32_t)(above < k ? key : INT32_MAX), [](uint32_t p, uint32_t q) { return (uint32_t)min((int32_t)p, (int32_t)q); });
+}
+
+// the k best of `count` entries (key kNoKey: none), by one wavefront
+template <typename Get>
+__device__ __forceinline__ Best best_of(uint32_t count, uint32_t k, Get get) {
+  Best b;
+  best_init(b);
+  int32_t most = kNoKey;
+#pragma unroll 4
+  for (uint32_t e = lane_id(); e < count; e += 64) most = max(most, get(e).x);
+  b.floor = kth_of_lanes(most, k);
+  for (uint32_t e0 = 0; e0 < count; e0 += 64) {
+    const uint32_t e = e0 + lane_id();
+    const int2 q = e < count ? get(e) : make_int2(kNoKey, INT32_MAX);
+    best_offer(b, q.x >= b.floor ? q.x : kNoKey, q.y, k);
+  }
+  return b;
+}
+
 template <int W, int V>
 __device__ __forceinline__ void feed_top(const float (&v)[W][V], uint32_t base, uint32_t stride, uint32_t C, Best &b, uint32_t k) {
 #pragma unroll
@@ -225,7 +274,10 @@ __device__ __forceinline__ void feed_top(const float (&v)[W][V], uint32_t base, 
     const uint32_t c = base + w * stride;
     if (!__any(c < C && !(m < b.thr))) continue;                // (uniform) nothing of this word reaches the k-th
 #pragma unroll
-    for (int j = 0; j < V; j++) best_offer(b, c + j < C ? key_of(v[w][j]) : kNoKey, (int32_t)(c + j), k);
+    for (int j = 0; j < V; j++) {
+      const int32_t key = key_of(v[w][j]);
+      best_offer(b, c + j < C && key >= b.floor ? key : kNoKey, (int32_t)(c + j), k);
+    }
   }
 }
 
@@ -235,7 +287,7 @@ template <typename T>
 __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
   constexpr int V = kVec<T>, W = kStreamWords, NW = kStreamThreads / 64;
   __shared__ float st[NW][3];
-  __shared__ int2 lists[NW][kMaxTop];
+  __shared__ int2 lists[NW * kMaxTop];
   const uint64_t row = blockIdx.x / a.splits;
   const uint32_t split = blockIdx.x % a.splits;
   const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.ldx;
@@ -259,6 +311,15 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
     feed_stats<W, V>(v, M, S, Tt);
     // (words past w1 are padding here: their index is put past C)
     if (a.k) {
+      if (w == w0) {                                            // (uniform) the first trip
+        float best = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < W; i++)
+#pragma unroll
+          for (int j = 0; j < V; j++) best = nan_max(best, v[i][j]);
+        b.floor = kth_of_lanes(w + threadIdx.x < w1 ? key_of(best) : kNoKey, a.k);
+        best_quick(b);
+      }
 #pragma unroll
       for (int i = 0; i < W; i++) {
         const uint32_t c = w + i * kStreamThreads + threadIdx.x;
@@ -280,24 +341,22 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
   for (int off = 1; off < 64; off <<= 1)
     join_stats(M, S, Tt, __shfl_xor(M, off, 64), __shfl_xor(S, off, 64), __shfl_xor(Tt, off, 64));
   if (lane_id() == 0) { st[wave_id()][0] = M; st[wave_id()][1] = S; st[wave_id()][2] = Tt; }
-  if (lane_id() < a.k) lists[wave_id()][lane_id()] = make_int2(b.key, b.idx);
+  if (a.splits > 1) {                         // (the wavefronts' lists go to the join as they are)
+    if (lane_id() < a.k) a.part_top[((row * a.splits + split) * NW + wave_id()) * a.k + lane_id()] = make_int2(b.key, b.idx);
+  } else if (lane_id() < a.k) {
+    lists[wave_id() * a.k + lane_id()] = make_int2(b.key, b.idx);
+  }
   __syncthreads();
   if (wave_id() != 0) return;
-  for (int w = 1; w < NW; w++) {
-    join_stats(M, S, Tt, st[w][0], st[w][1], st[w][2]);
-    if (a.k) {
-      const int2 e = lane_id() < a.k ? lists[w][lane_id()] : make_int2(kNoKey, INT32_MAX);
-      best_offer(b, e.x, e.y, a.k);
-    }
-  }
+  for (int w = 1; w < NW; w++) join_stats(M, S, Tt, st[w][0], st[w][1], st[w][2]);
   if (a.splits > 1) {
     if (lane_id() == 0) {
       float *p = a.part + (row * a.splits + split) * 4;
       p[0] = M; p[1] = S; p[2] = Tt;
     }
-    if (lane_id() < a.k) a.part_top[(row * a.splits + split) * a.k + lane_id()] = make_int2(b.key, b.idx);
     return;
   }
+  if (a.k) b = best_of(NW * a.k, a.k, [&](uint32_t e) { return lists[e]; });
   float H;
   const float2 stat = finish_stats(M, S, Tt, H);
   if (lane_id() == 0) answer_row(a, row, x, stat, H);
@@ -307,11 +366,22 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
   }
 }
 
-// joins the splits of a row: one wavefront per row
+// joins the splits of a row: one workgroup per row, each wavefront a quarter of the lists
 template <typename T>
-__global__ void __launch_bounds__(64) lp_join_kernel(LpArgs a) {
+__global__ void __launch_bounds__(kStreamThreads) lp_join_kernel(LpArgs a) {
+  constexpr uint32_t NW = kStreamThreads / 64;
+  __shared__ int2 lists[NW * kMaxTop];
   const uint64_t row = blockIdx.x;
+  if (a.k) {
+    const uint32_t count = a.splits * a.k;    // (a quarter: as many lists as there are splits)
+    const int2 *mine = a.part_top + (row * NW + wave_id()) * count;
+    const Best b = best_of(count, a.k, [&](uint32_t e) { return mine[e]; });
+    if (lane_id() < a.k) lists[wave_id() * a.k + lane_id()] = make_int2(b.key, b.idx);
+    __syncthreads();
+  }
+  if (wave_id() != 0) return;
   float M = -INFINITY, S = 0.f, Tt = 0.f;
+#pragma unroll 4
   for (uint32_t s = lane_id(); s < a.splits; s += 64) {
     const float *p = a.part + (row * a.splits + s) * 4;
     join_stats(M, S, Tt, p[0], p[1], p[2]);
@@ -323,14 +393,7 @@ __global__ void __launch_bounds__(64) lp_join_kernel(LpArgs a) {
   const float2 stat = finish_stats(M, S, Tt, H);
   if (lane_id() == 0) answer_row(a, row, static_cast<const T *>(a.x) + (int64_t)row * a.ldx, stat, H);
   if (!a.k) return;
-  Best b;
-  best_init(b);
-  const uint32_t total = a.splits * a.k;
-  for (uint32_t e0 = 0; e0 < total; e0 += 64) {
-    const uint32_t e = e0 + lane_id();
-    const int2 q = e < total ? a.part_top[row * total + e] : make_int2(kNoKey, INT32_MAX);
-    best_offer(b, q.x, q.y, a.k);
-  }
+  const Best b = best_of(NW * a.k, a.k, [&](uint32_t e) { return lists[e]; });
   if (lane_id() < a.k) {
     a.top_lp[row * a.k + lane_id()] = logprob_of(value_of(b.key), stat);
     a.top_idx[row * a.k + lane_id()] = b.idx;
@@ -445,14 +508,16 @@ void rows_dispatch(const LpArgs &a, hipStream_t st) {
 template <typename T>
 void stream_launch(const LpArgs &a, hipStream_t st) {
   hipLaunchKernelGGL((lp_stream_kernel<T>), dim3(a.n * a.splits), dim3(kStreamThreads), 0, st, a);
-  if (a.splits > 1) hipLaunchKernelGGL((lp_join_kernel<T>), dim3(a.n), dim3(64), 0, st, a);
+  if (a.splits > 1) hipLaunchKernelGGL((lp_join_kernel<T>), dim3(a.n), dim3(kStreamThreads), 0, st, a);
 }
 
 template <typename T, int V>
 void bwd_launch(const LpBwdArgs &a, hipStream_t st) {
   const uint32_t nch = a.C / V;
+  // lanes of a row: four trips each (the power of two that covers a row of 43 words leaves a third of its lanes idle: 100 us for
+  // 289127 rows of 172 fp32)
   uint32_t lanes = 4;
-  while (lanes < nch && lanes < 256) lanes <<= 1;
+  while (lanes * 4 < nch && lanes < 256) lanes <<= 1;
   // a long row is cut into parts of 8 trips, so that few rows still fill the chip
   const uint32_t per = lanes * 8, parts = (nch + per - 1) / per;
   const uint64_t need = ((uint64_t)a.n * parts + 256 / lanes - 1) / (256 / lanes);
@@ -471,7 +536,7 @@ int check(const char *who, int dtype, uint32_t n, uint32_t C, uint32_t k) {
 extern "C" size_t sl_label_logprobs_scratch_bytes(int dtype, uint32_t n, uint32_t C, uint32_t k) {
   if (!elem_dtype_ok(dtype) || n == 0 || C == 0 || k > kMaxTop || forward_in_registers(C)) return 0;
   const uint32_t s = splits_of(n, C, dtype);
-  return s > 1 ? (size_t)n * s * (16 + 8 * (size_t)k) : 0;
+  return s > 1 ? (size_t)n * s * (16 + 8 * (kStreamThreads / 64) * (size_t)k) : 0;
 }
 
 extern "C" int sl_label_logprobs_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_label, int label_i64, uint32_t n, uint32_t C,

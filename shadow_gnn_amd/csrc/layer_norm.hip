@@ -27,7 +27,8 @@ struct LnArgs {
   // backward
   const void *dy;
   int64_t lddy;
-  float *partial;                          // [gridDim.x, 2, F]
+  float *partial;                          // [gridDim.x, 2, F]; null with one workgroup, which writes dscale / doffset
+  void *dscale, *doffset;
 };
 
 template <typename T, int V>
@@ -173,16 +174,23 @@ __global__ void __launch_bounds__(L < 256 ? 256 : L) ln_bwd_kernel(LnArgs a) {
       }
     }
   }
-  if (!a.partial) return;
+  if (!a.partial && !a.dscale && !a.doffset) return;
   // one row of partial sums per workgroup: over the row groups of a wavefront, then over its wavefronts, in a fixed order
-  float *out = a.partial + (uint64_t)blockIdx.x * 2 * a.F;
+  auto put = [&](int q, uint32_t f, float t) {
+    if (a.partial) {
+      a.partial[((uint64_t)blockIdx.x * 2 + q) * a.F + f] = t;
+    } else if (void *w = q ? a.doffset : a.dscale) {
+      if (a.w_f32) static_cast<float *>(w)[f] = t;
+      else static_cast<T *>(w)[f] = (T)t;
+    }
+  };
   if (L > 64) {
 #pragma unroll
     for (int i = 0; i < NC; i++) {
       const uint32_t c = sub + i * L;
       if (c < nch) {
 #pragma unroll
-        for (int j = 0; j < V; j++) { out[c * V + j] = ds[i][j]; out[a.F + c * V + j] = dof[i][j]; }
+        for (int j = 0; j < V; j++) { put(0, c * V + j, ds[i][j]); put(1, c * V + j, dof[i][j]); }
       }
     }
     return;
@@ -210,7 +218,7 @@ __global__ void __launch_bounds__(L < 256 ? 256 : L) ln_bwd_kernel(LnArgs a) {
       float t = 0.f;
 #pragma unroll
       for (int w = 0; w < T_ / 64; w++) t += lds[(w * 2 + q) * (L * kElems) + f];
-      out[q * a.F + f] = t;
+      put(q, f, t);
     }
   }
 }
@@ -246,11 +254,15 @@ int lanes_of(uint32_t F) {
   return 1024;
 }
 
+// up to this many trips one workgroup takes all rows and writes the weight gradient itself: a launch (some 4 us of the host's time)
+// less than it costs
+constexpr uint32_t kAlone = 4;
+
 uint32_t bwd_blocks(uint32_t n, uint32_t F) {
   const int L = lanes_of(F);
   const uint32_t G = L < 256 ? 256 / L : 1, need = (uint32_t)(((uint64_t)n + G - 1) / G);
   const uint32_t most = L == 1024 ? 256u : 1024u;
-  return need < most ? need : most;
+  return need <= kAlone ? 1u : need < most ? need : most;
 }
 
 template <typename T, int V>
@@ -298,7 +310,9 @@ int check_shape(const char *who, int dtype, int w_dtype, uint32_t F) {
 }  // namespace
 
 extern "C" size_t sl_layer_norm_partial_floats(uint32_t n, uint32_t F) {
-  return F >= 1 && F <= kMaxF ? (size_t)bwd_blocks(n, F) * 2 * F : 0;
+  if (F < 1 || F > kMaxF || n == 0) return 0;
+  const uint32_t b = bwd_blocks(n, F);
+  return b > 1 ? (size_t)b * 2 * F : 0;
 }
 
 extern "C" int sl_layer_norm_fwd(int dtype, int w_dtype, const void *d_x, int64_t ldx, const void *d_scale, const void *d_offset, uint32_t n,
@@ -323,20 +337,22 @@ extern "C" int sl_layer_norm_bwd(int dtype, int w_dtype, const void *d_x, int64_
                                  float *d_partial, void *stream) {
   if (const int rc = check_shape("sl_layer_norm_bwd", dtype, w_dtype, F)) return rc;
   const bool weights = d_dscale || d_doffset;
-  if (n && (!d_x || !d_dy || !d_stats || ldx < (int64_t)F || lddy < (int64_t)F || (d_dx && lddx < (int64_t)F) || (weights && !d_partial)))
+  if (n && (!d_x || !d_dy || !d_stats || ldx < (int64_t)F || lddy < (int64_t)F || (d_dx && lddx < (int64_t)F) || (weights && !d_partial && bwd_blocks(n, F) > 1)))
     return set_error(SG_ERR_INVALID, "sl_layer_norm_bwd: operands");
   hipStream_t st = (hipStream_t)stream;
   const uint32_t grid = n ? bwd_blocks(n, F) : 0;
+  const bool alone = grid == 1;
   if (n && (d_dx || weights)) {
     LnArgs a = {};
     a.x = d_x; a.dy = d_dy; a.scale = d_scale; a.y = d_dx; a.ldx = ldx; a.lddy = lddy; a.ldy = lddx; a.stats = const_cast<float *>(d_stats);
-    a.n = n; a.F = F; a.w_f32 = w_dtype == SL_F32; a.partial = weights ? d_partial : nullptr;
+    a.n = n; a.F = F; a.w_f32 = w_dtype == SL_F32; a.partial = weights && !alone ? d_partial : nullptr;
+    if (alone) { a.dscale = d_dscale; a.doffset = d_doffset; }
     SHD_PROF_FMT((double)3 * n * F * elem_bytes(dtype), 0, st, "layer_norm_bwd_F%u", F);
     const bool words = rows_of_words(d_x, ldx, F, dtype) && rows_of_words(d_dy, lddy, F, dtype) && rows_of_words(d_dx, lddx, F, dtype);
     SHD_DISPATCH_ELEM(dtype, if (words) bwd_launch<T, kVec<T>>(a, st); else bwd_launch<T, 1>(a, st));
     SHD_HIP(hipGetLastError());
   }
-  if (weights) {
+  if (weights && !alone) {
     const dim3 g((2 * F + 31) / 32), b(1024);
     SHD_DISPATCH_ELEM(w_dtype, hipLaunchKernelGGL((ln_wgrad_kernel<T>), g, b, 0, st, d_partial, grid, F, (T *)d_dscale, (T *)d_doffset));
     SHD_HIP(hipGetLastError());

@@ -157,7 +157,8 @@ struct LayerNorm : public Function<LayerNorm> {
       if (need_s) out[1] = like(scale, scale.sizes());
       if (need_o) out[2] = like(offset, offset.sizes());
       Tensor part;
-      if (need_s || need_o) part = like(x, {(int64_t)sl_layer_norm_partial_floats(n, F) + 1}, at::kFloat);
+      const int64_t floats = need_s || need_o ? (int64_t)sl_layer_norm_partial_floats(n, F) : 0;
+      if (floats) part = like(x, {floats}, at::kFloat);
       const Tensor &w = scale.defined() ? scale : offset;
       const On on(x);
       check(sl_layer_norm_bwd(dtype_of(x), w.defined() ? dtype_of(w) : SL_F32, r.p, r.ld, d.p, d.ld, ptr(scale), (const float *)stats.data_ptr(), n, F,
