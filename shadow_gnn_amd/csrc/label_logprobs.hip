@@ -247,15 +247,56 @@ __device__ __forceinline__ int32_t kth_of_lanes(int32_t key, uint32_t k) {
   return (int32_t)group_all<64>((uint32_t)(above < k ? key : INT32_MAX), [](uint32_t p, uint32_t q) { return (uint32_t)min((int32_t)p, (int32_t)q); });
 }
 
-// the k best of `count` entries (key kNoKey: none), by one wavefront
+// Collects candidates of a wavefront into 64 places of LDS; more than 64 do not fit (the caller then offers them one by one).
+struct Collect {
+  int2 *place;
+  uint32_t total;
+};
+__device__ __forceinline__ void collect(Collect &c, bool valid, int32_t key, int32_t idx) {
+  const uint64_t mask = __ballot(valid);
+  const uint32_t pos = c.total + (uint32_t)__popcll(mask & lanemask_lt());
+  if (valid && pos < 64) c.place[pos] = make_int2(key, idx);
+  c.total += (uint32_t)__popcll(mask);
+}
+// ... and makes them the list: every candidate's rank is the number that beat it (all distinct).  An insertion costs some 180 ns, this
+// 0.5 us for fifteen of them.
+__device__ __forceinline__ void rank_collected(const Collect &c, Best &b, uint32_t k) {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint32_t lane = lane_id();
+  const int2 q = lane < c.total ? c.place[lane] : make_int2(kNoKey, INT32_MAX);
+  uint32_t rank = 0;
+  for (uint32_t l = 0; l < c.total; l++)
+    rank += better(__builtin_amdgcn_readlane(q.x, (int)l), __builtin_amdgcn_readlane(q.y, (int)l), q.x, q.y) ? 1u : 0u;
+  if (lane < c.total) c.place[rank] = q;      // (each has been read)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int2 e = lane < c.total && lane < k ? c.place[lane] : make_int2(kNoKey, INT32_MAX);
+  b.key = e.x; b.idx = e.y;
+  b.thr_key = __builtin_amdgcn_readlane(b.key, (int)k - 1);
+  b.thr_idx = __builtin_amdgcn_readlane(b.idx, (int)k - 1);
+  best_quick(b);
+}
+
+// the k best of `count` entries (key kNoKey: none), by one wavefront; place: 64 entries of LDS of its own
 template <typename Get>
-__device__ __forceinline__ Best best_of(uint32_t count, uint32_t k, Get get) {
+__device__ __forceinline__ Best best_of(uint32_t count, uint32_t k, int2 *place, Get get) {
   Best b;
   best_init(b);
   int32_t most = kNoKey;
 #pragma unroll 4
   for (uint32_t e = lane_id(); e < count; e += 64) most = max(most, get(e).x);
   b.floor = kth_of_lanes(most, k);
+  Collect c = {place, 0};
+  for (uint32_t e0 = 0; e0 < count; e0 += 64) {
+    const uint32_t e = e0 + lane_id();
+    const int2 q = e < count ? get(e) : make_int2(kNoKey, INT32_MAX);
+    collect(c, q.x != kNoKey && q.x >= b.floor, q.x, q.y);
+  }
+  if (c.total <= 64) {
+    rank_collected(c, b, k);
+    return b;
+  }
   for (uint32_t e0 = 0; e0 < count; e0 += 64) {
     const uint32_t e = e0 + lane_id();
     const int2 q = e < count ? get(e) : make_int2(kNoKey, INT32_MAX);
@@ -287,7 +328,7 @@ template <typename T>
 __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
   constexpr int V = kVec<T>, W = kStreamWords, NW = kStreamThreads / 64;
   __shared__ float st[NW][3];
-  __shared__ int2 lists[NW * kMaxTop];
+  __shared__ int2 lists[NW * kMaxTop], places[NW][64];
   const uint64_t row = blockIdx.x / a.splits;
   const uint32_t split = blockIdx.x % a.splits;
   const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.ldx;
@@ -319,6 +360,20 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
           for (int j = 0; j < V; j++) best = nan_max(best, v[i][j]);
         b.floor = kth_of_lanes(w + threadIdx.x < w1 ? key_of(best) : kNoKey, a.k);
         best_quick(b);
+        Collect col = {places[wave_id()], 0};
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const uint32_t c = w + i * kStreamThreads + threadIdx.x;
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            const int32_t key = key_of(v[i][j]);
+            collect(col, c < w1 && key >= b.floor, key, (int32_t)(head + c * V + j));
+          }
+        }
+        if (col.total <= 64) {
+          rank_collected(col, b, a.k);
+          continue;
+        }
       }
 #pragma unroll
       for (int i = 0; i < W; i++) {
@@ -356,7 +411,7 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
     }
     return;
   }
-  if (a.k) b = best_of(NW * a.k, a.k, [&](uint32_t e) { return lists[e]; });
+  if (a.k) b = best_of(NW * a.k, a.k, places[0], [&](uint32_t e) { return lists[e]; });
   float H;
   const float2 stat = finish_stats(M, S, Tt, H);
   if (lane_id() == 0) answer_row(a, row, x, stat, H);
@@ -370,12 +425,12 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kStreamThreads) lp_join_kernel(LpArgs a) {
   constexpr uint32_t NW = kStreamThreads / 64;
-  __shared__ int2 lists[NW * kMaxTop];
+  __shared__ int2 lists[NW * kMaxTop], places[NW][64];
   const uint64_t row = blockIdx.x;
   if (a.k) {
     const uint32_t count = a.splits * a.k;    // (a quarter: as many lists as there are splits)
     const int2 *mine = a.part_top + (row * NW + wave_id()) * count;
-    const Best b = best_of(count, a.k, [&](uint32_t e) { return mine[e]; });
+    const Best b = best_of(count, a.k, places[wave_id()], [&](uint32_t e) { return mine[e]; });
     if (lane_id() < a.k) lists[wave_id() * a.k + lane_id()] = make_int2(b.key, b.idx);
     __syncthreads();
   }
@@ -393,7 +448,7 @@ __global__ void __launch_bounds__(kStreamThreads) lp_join_kernel(LpArgs a) {
   const float2 stat = finish_stats(M, S, Tt, H);
   if (lane_id() == 0) answer_row(a, row, static_cast<const T *>(a.x) + (int64_t)row * a.ldx, stat, H);
   if (!a.k) return;
-  const Best b = best_of(NW * a.k, a.k, [&](uint32_t e) { return lists[e]; });
+  const Best b = best_of(NW * a.k, a.k, places[0], [&](uint32_t e) { return lists[e]; });
   if (lane_id() < a.k) {
     a.top_lp[row * a.k + lane_id()] = logprob_of(value_of(b.key), stat);
     a.top_idx[row * a.k + lane_id()] = b.idx;
