@@ -106,23 +106,44 @@ constexpr int kStage = 2 * kTileBytes;
 
 __device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
 
-// 16 bytes at any alignment; elements at and past `left` read as zero
+// Eight elements from column c of a row of `width`, at any alignment; those past the row's end are zero.
+// Rows of eight and more: fetched without a branch -- where the row ends inside the word, as the 16 bytes that end with it -- and shifted
+// down when used, so that the loads of a stage are on their way together (behind a branch each, they waited for one another: 25 instead
+// of 17 us at 20011 x 500 x 47).  Narrower rows: element by element.
 template <typename T>
-__device__ __forceinline__ uint4 load_word(const T *p, int left) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (left >= 8) {
-    __builtin_memcpy(&v, p, 16);
-  } else if (left > 0) {
-    uint16_t h[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) h[j] = 0;
-#pragma unroll
-    for (int j = 0; j < 7; j++)
-      if (j < left) __builtin_memcpy(&h[j], p + j, 2);
-    __builtin_memcpy(&v, h, 16);
-  }
+__device__ __forceinline__ uint4 fetch_word(const T *row, uint32_t c, uint32_t width) {
+  uint4 v;
+  __builtin_memcpy(&v, row + min(c, width - 8), 16);
   return v;
 }
+__device__ __forceinline__ uint4 settle_word(const uint4 &v, uint32_t c, uint32_t width) {
+  const uint32_t back = c + 8 > width ? c + 8 - width : 0, sh = (back & 3) * 16;
+  uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+  lo = back & 4 ? hi : lo;
+  hi = back & 4 ? 0 : hi;
+  lo = lo >> sh | (hi << 1) << (63 - sh);
+  hi >>= sh;
+  const uint32_t keep = back >= 8 ? 0u : 0xFFFFFFFFu;
+  return make_uint4((uint32_t)lo & keep, (uint32_t)(lo >> 32) & keep, (uint32_t)hi & keep, (uint32_t)(hi >> 32) & keep);
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_elems(const T *row, uint32_t c, uint32_t width) {
+  uint4 v;
+  uint16_t h[8];
+#pragma unroll
+  for (uint32_t j = 0; j < 8; j++) {
+    h[j] = 0;
+    if (c + j < width) __builtin_memcpy(&h[j], row + c + j, 2);
+  }
+  __builtin_memcpy(&v, h, 16);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_word(const T *row, uint32_t c, uint32_t width) {
+  return width < 8 ? load_elems(row, c, width) : settle_word(fetch_word(row, c, width), c, width);
+}
+// how an operand's rows are read
+enum Via { kWords, kRegs, kElems };          // whole 16-byte words; rows of eight elements and more; any rows
 
 // everything this wavefront has sent to LDS has arrived, and everybody's has
 __device__ __forceinline__ void stage_barrier() {
@@ -186,9 +207,9 @@ __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t word) { return wo
 template <typename T, int ROWS, int THREADS, bool DIRECT>
 struct KLoader {
   static constexpr int P = ROWS * 8 / THREADS;
-  const char *base;                          // the tile's first row at the next stage's first column (uniform)
-  uint32_t off[P];                           // this thread's words from there, in bytes (the host keeps the pitch below 2^22 elements)
-  uint32_t k;                                // the stage's first column
+  const char *base;                          // the tile's first row (DIRECT: at the next stage's first column); uniform
+  uint32_t off[P];                           // this thread's rows (DIRECT: words) from there, in bytes (the host keeps the pitch below 2^22 elements)
+  uint32_t k;                                // the next stage's first column
   uint32_t K;
   uint4 reg[DIRECT ? 1 : P];
 
@@ -199,7 +220,7 @@ struct KLoader {
 #pragma unroll
     for (int i = 0; i < P; i++) {            // (rows past the end repeat the last one: their products are not stored)
       const uint32_t r = (i * THREADS + threadIdx.x) >> 3;
-      off[i] = (min(r0 + r, rows - 1) - r0) * (uint32_t)ld * 2 + col(i) * 2;
+      off[i] = (min(r0 + r, rows - 1) - r0) * (uint32_t)ld * 2 + (DIRECT ? col(i) * 2 : 0);
     }
   }
   // transfer i of the next stage
@@ -207,17 +228,24 @@ struct KLoader {
     if (k + 64 <= K) lds_dma16_async(base, off[i], lds + i * THREADS * 16);
     else lds_dma16_async(k + col(i) < K ? (const void *)(base + off[i]) : (const void *)g_zero16, lds + i * THREADS * 16);      // (K % 8 == 0)
   }
-  __device__ __forceinline__ void next() { base += 128; k += 64; }
-  __device__ __forceinline__ void start(uint32_t lds) {
+  __device__ __forceinline__ void next() {
+    if (DIRECT) base += 128;
+    k += 64;
+  }
+  // the next stage into registers (K >= 8), and from there to LDS
+  __device__ __forceinline__ void fetch() {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int i = 0; i < P; i++) {
-      if constexpr (DIRECT) send(i, lds);
-      else reg[i] = load_word(reinterpret_cast<const T *>(base + off[i]), (int)K - (int)(k + col(i)));
+      for (int i = 0; i < P; i++) reg[i] = fetch_word(reinterpret_cast<const T *>(base + off[i]), k + col(i), K);
+      next();
     }
-    next();
   }
   __device__ __forceinline__ void finish(char *lds) {
     if constexpr (!DIRECT) {
+      if (k > K) {                           // (k is past the stage that was fetched: it is the last, and the rows end inside it)
+#pragma unroll
+        for (int i = 0; i < P; i++) reg[i] = settle_word(reg[i], k - 64 + col(i), K);
+      }
 #pragma unroll
       for (int i = 0; i < P; i++) *reinterpret_cast<uint4 *>(lds + (i * THREADS + threadIdx.x) * 16) = reg[i];
     }
@@ -368,11 +396,11 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
     if constexpr (!DIRECT) {
       la.init(a.A, a.lda, m0, a.M, a.K);
       lb.init(a.B, a.ldb, n0, a.N, a.K);
-      la.start(0); lb.start(0);
+      la.fetch(); lb.fetch();
       __syncthreads();                       // (the tile before has been read)
       at = 0;
       la.finish(lds); lb.finish(lds + kA);
-      if (steps > 1) { la.start(0); lb.start(0); }
+      if (steps > 1) { la.fetch(); lb.fetch(); }
       __syncthreads();
       read_quarter(lds, 0);
     }
@@ -384,7 +412,7 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
         if constexpr (!DIRECT) {
           if (q == 0 && s + 1 < steps) {     // (the next stage's place was last read before the previous barrier)
             la.finish(lds + nx * kBoth); lb.finish(lds + nx * kBoth + kA);
-            if (s + 2 < steps) { la.start(0); lb.start(0); }
+            if (s + 2 < steps) { la.fetch(); lb.fetch(); }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -441,9 +469,10 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
     float b[8];
     load_bias<T>(a, n, left, b);
     uint32_t m = m0 + wm + er;               // this lane's next row
-    const T *res = static_cast<const T *>(a.res) + (int64_t)m * a.ldr + n;
+    const T *res = static_cast<const T *>(a.res) + (int64_t)m * a.ldr;
+    const bool res_ahead = a.res && a.N >= 8;
     uint4 next = make_uint4(0, 0, 0, 0);
-    if (a.res && m < a.M) next = load_word(res, left);
+    if (res_ahead && m < a.M) next = fetch_word(res, n, a.N);
 #pragma unroll
     for (int j = 0; j < MI; j++) {
 #pragma unroll 1
@@ -460,14 +489,15 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
 #pragma unroll 1
         for (uint32_t p = 0; p < 16; p += 8, m += 8) {
           const uint4 resw = next;
+          const T *here = res;
           res += 8 * a.ldr;
-          if (a.res && m + 8 < a.M) next = load_word(res, left);       // (a pass ahead; past the wavefront's last row it is not used)
+          if (res_ahead && m + 8 < a.M) next = fetch_word(res, n, a.N);      // (a pass ahead; past the wavefront's last row it is not used)
           if (m < a.M && left > 0) {
             const uint32_t r = p + er;
             float v[8];
             *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2) ^ r) * 4);
             *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2 + 1) ^ r) * 4);
-            finish8<T>(a, m, n, left, v, b, resw);
+            finish8<T>(a, m, n, left, v, b, !a.res ? resw : res_ahead ? settle_word(resw, n, a.N) : load_elems(here, n, a.N));
           }
         }
         wave_order();
@@ -478,7 +508,7 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
 
 // Few output tiles: 32 x 32 tiles, the contraction cut over the workgroup's eight wavefronts (step 16 w, 16 (w + 8), ...), their
 // products joined in LDS in wavefront order.  Operands go from memory to the product's registers: every word is used once.
-template <typename T, bool WORDS>
+template <typename T, Via VIA>
 __global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
   typedef typename Frag<T>::v8 v8;
   constexpr int kPitch = 36;
@@ -496,18 +526,26 @@ __global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
-      if (WORDS) {
+      if (VIA == kWords) {
         const bool in = k < a.K;
         wa[u] = in ? *reinterpret_cast<const uint4 *>(pa + k) : make_uint4(0, 0, 0, 0);
         wb[u] = in ? *reinterpret_cast<const uint4 *>(pb + k) : make_uint4(0, 0, 0, 0);
+      } else if (VIA == kRegs) {
+        wa[u] = fetch_word(pa, k, a.K);
+        wb[u] = fetch_word(pb, k, a.K);
       } else {
-        wa[u] = load_word(pa + k, (int)a.K - (int)k);
-        wb[u] = load_word(pb + k, (int)a.K - (int)k);
+        wa[u] = load_elems(pa, k, a.K);
+        wb[u] = load_elems(pb, k, a.K);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       v8 fa, fb;
+      if (VIA == kRegs) {
+        const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
+        wa[u] = settle_word(wa[u], k, a.K);
+        wb[u] = settle_word(wb[u], k, a.K);
+      }
       __builtin_memcpy(&fa, &wa[u], 16);
       __builtin_memcpy(&fb, &wb[u], 16);
       acc = mma(fb, fa, acc);
@@ -529,7 +567,7 @@ __global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] += part[w][er * kPitch + ec + e];
   uint4 resw = make_uint4(0, 0, 0, 0);
-  if (a.res) resw = load_word(static_cast<const T *>(a.res) + (int64_t)m * a.ldr + n, left);
+  if (a.res) resw = load_word(static_cast<const T *>(a.res) + (int64_t)m * a.ldr, n, a.N);
   float b[8];
   load_bias<T>(a, n, left, b);
   finish8<T>(a, m, n, left, v, b, resw);
@@ -750,26 +788,32 @@ struct TnArgs {
 // the LDS image of a stage: 64 rows of the contraction x 128 columns (256 bytes); 16-byte word w of row r sits at w ^ (2 (r & 3) | 8 ((r >> 2) & 1))
 __device__ __forceinline__ uint32_t swz_t(uint32_t row, uint32_t word) { return word ^ ((row & 3) * 2 + ((row >> 2) & 1) * 8); }
 
-template <typename T, bool DIRECT>
+template <typename T, Via VIA>
 struct RowLoader {
-  const T *base;                             // column c0 of row 0
+  const T *base;                             // row 0 of the operand
   int64_t ld;
-  int cols;                                  // valid columns from c0 on (>= 1)
-  uint4 reg[4];
+  uint32_t c0, width;                        // the tile's first column; columns of the operand
+  uint32_t past;                             // rows fetched that do not exist (the slice's last stage): from row `past` of the stage on
+  uint4 reg[VIA == kWords ? 1 : 4];
   __device__ __forceinline__ void start(uint32_t r0, uint32_t r1, char *lds) {       // rows r0 .. r0 + 63, those at and past r1 read as zero
+    past = r1 - r0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t w = i * kThreads + threadIdx.x, r = w >> 4, c = swz_t(r, w & 15) * 8;
-      const bool in = r0 + r < r1 && (int)c < cols;
-      const T *p = base + (int64_t)(r0 + r) * ld + c;
-      if (DIRECT) lds_dma16(in ? (const void *)p : (const void *)g_zero16, lds + (i * kThreads + (threadIdx.x & ~63u)) * 16);
-      else reg[i] = in ? load_word(p, cols - (int)c) : make_uint4(0, 0, 0, 0);
+      const uint32_t w = i * kThreads + threadIdx.x, r = w >> 4, c = c0 + swz_t(r, w & 15) * 8;
+      const T *row = base + (int64_t)min(r0 + r, r1 - 1) * ld;
+      if (VIA == kWords) lds_dma16(r0 + r < r1 && c < width ? (const void *)(row + c) : (const void *)g_zero16, lds + (i * kThreads + (threadIdx.x & ~63u)) * 16);
+      else if (VIA == kRegs) reg[i] = fetch_word(row, c, width);
+      else reg[i] = load_elems(row, c, width);
     }
   }
   __device__ __forceinline__ void finish(char *lds) {
-    if (!DIRECT) {
+    if (VIA != kWords) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(lds + (i * kThreads + threadIdx.x) * 16) = reg[i];
+      for (int i = 0; i < 4; i++) {
+        const uint32_t w = i * kThreads + threadIdx.x, r = w >> 4;
+        if (VIA == kRegs && c0 + 128 > width) reg[i] = settle_word(reg[i], c0 + swz_t(r, w & 15) * 8, width);
+        *reinterpret_cast<uint4 *>(lds + w * 16) = r < past ? reg[i] : make_uint4(0, 0, 0, 0);
+      }
     }
   }
 };
@@ -790,7 +834,7 @@ __device__ __forceinline__ typename Frag<T>::v8 read_cols(const char *img, uint3
   return u.v;
 }
 
-template <typename T, bool DA, bool DB>
+template <typename T, Via DA, Via DB>
 __global__ void __launch_bounds__(kThreads, 2) tn_kernel(TnArgs a) {
   typedef typename Frag<T>::v8 v8;
   __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
@@ -802,8 +846,8 @@ __global__ void __launch_bounds__(kThreads, 2) tn_kernel(TnArgs a) {
   const uint32_t r0 = slice * a.per, r1 = min(a.M, r0 + a.per);
   RowLoader<T, DA> la;
   RowLoader<T, DB> lb;
-  la.base = static_cast<const T *>(a.A) + n0; la.ld = a.lda; la.cols = (int)min((uint32_t)BN, a.N - n0);
-  lb.base = static_cast<const T *>(a.B) + k0; lb.ld = a.ldb; lb.cols = (int)min((uint32_t)BM, a.K - k0);
+  la.base = static_cast<const T *>(a.A); la.ld = a.lda; la.c0 = n0; la.width = a.N;
+  lb.base = static_cast<const T *>(a.B); lb.ld = a.ldb; lb.c0 = k0; lb.width = a.K;
   const bool with_b = a.part_b && tk == 0 && (wave & 1) == 0;           // (uniform over the wavefront)
   f32x16 acc[2][2], accb[2];                 // [n half][k half]
 #pragma unroll
@@ -976,24 +1020,28 @@ __global__ void __launch_bounds__(NB * KB * 64, 2) tn_narrow_kernel(TnNarrowArgs
     }
 }
 
-// sums of the slices in slice order: the first N K threads dW (part null: it is written already), N more db (part_b null: not wanted)
+// Sums of the slices: 64 outputs per workgroup, each of its four wavefronts every fourth slice, joined in wavefront order (always the
+// same order).  The first N K outputs are dW (part null: it is written already), N more db (part_b null: not wanted).
 template <typename T>
 __global__ void __launch_bounds__(256) tn_join_kernel(const float *__restrict__ part, const float *__restrict__ part_b, uint32_t slices, uint32_t N,
                                                       uint32_t K, T *C, int64_t ldc, void *db, int db_f32) {
+  __shared__ float sums[4][64];
   const uint64_t total = part ? (uint64_t)N * K : 0;
-  uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint64_t o = (uint64_t)blockIdx.x * 64 + lane_id(), e = o < total ? o : o - total;
+  const bool in = o < total + (part_b ? N : 0);
+  const float *src = o < total ? part : part_b;
+  const uint64_t step = o < total ? total : N;
   float t = 0.f;
-  if (e < total) {
+  if (in) {
 #pragma unroll 8
-    for (uint32_t s = 0; s < slices; s++) t += part[s * total + e];
-    C[(int64_t)(e / K) * ldc + e % K] = (T)t;
-    return;
+    for (uint32_t s = wave_id(); s < slices; s += 4) t += src[s * step + e];
   }
-  e -= total;
-  if (!part_b || e >= N) return;
-#pragma unroll 8
-  for (uint32_t s = 0; s < slices; s++) t += part_b[(uint64_t)s * N + e];
-  if (db_f32) static_cast<float *>(db)[e] = t;
+  sums[wave_id()][lane_id()] = t;
+  __syncthreads();
+  if (wave_id() != 0 || !in) return;
+  t = (sums[0][lane_id()] + sums[1][lane_id()]) + (sums[2][lane_id()] + sums[3][lane_id()]);
+  if (o < total) C[(int64_t)(e / K) * ldc + e % K] = (T)t;
+  else if (db_f32) static_cast<float *>(db)[e] = t;
   else static_cast<T *>(db)[e] = (T)t;
 }
 
@@ -1006,7 +1054,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, cons
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
     const uint64_t m = i / words;
     const uint32_t w = (uint32_t)(i % words);
-    const uint4 g = load_word(dy + (int64_t)m * lddy + w * 8, (int)N - (int)w * 8);       // (zero past N)
+    const uint4 g = load_word(dy + (int64_t)m * lddy, w * 8, N);       // (zero past N)
     uint4 z = make_uint4(0, 0, 0, 0);
     if (keeps_bits(act)) z.x = (uint8_t)kept[m * pitch + w];
     else z = *reinterpret_cast<const uint4 *>(kept + m * pitch + w * 16);
@@ -1064,9 +1112,10 @@ template <typename T, int BM_, int BN_, int WM, int WN, int ST, int OCC, int PER
 void nt_tiles(GemmArgs a, bool direct, hipStream_t st) {
   a.tiles_m = (a.M + BM_ - 1) / BM_; a.tiles_n = (a.N + BN_ - 1) / BN_;
   const uint32_t tiles = a.tiles_m * a.tiles_n, most = 256 * PERCU;       // (a multiple of eight: a workgroup stays on its XCD's tiles)
-  const dim3 g(tiles < most ? tiles : most), b(WM * WN * 64);
-  if (direct) hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, ST, OCC, true>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), g, b, 0, st, a);
+  const dim3 b(WM * WN * 64);
+  // (nothing of the next tile is on its way in the form through registers: a workgroup per tile there)
+  if (direct) hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, ST, OCC, true>), dim3(tiles < most ? tiles : most), b, 0, st, a);
+  else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), dim3(tiles), b, 0, st, a);
 }
 
 template <typename T, int SIDE>
@@ -1108,14 +1157,16 @@ void nt_launch(GemmArgs a, hipStream_t st) {
     return;
   }
   const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
-  // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches are rare and take the other)
+  // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches and contractions of less
+  //  than eight are rare and take the other)
   // (fewer than 64 tiles of 128: 1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128 ones, twice the
   //  rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47)
-  if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22)) {
+  if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22) || a.K < 8) {
     a.tiles_m = (a.M + 31) / 32; a.tiles_n = (a.N + 31) / 32;
     const dim3 g(a.tiles_m * a.tiles_n), b(512);
-    if (direct) hipLaunchKernelGGL((nt_few_kernel<T, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((nt_few_kernel<T, false>), g, b, 0, st, a);
+    if (direct) hipLaunchKernelGGL((nt_few_kernel<T, kWords>), g, b, 0, st, a);
+    else if (a.K >= 8) hipLaunchKernelGGL((nt_few_kernel<T, kRegs>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((nt_few_kernel<T, kElems>), g, b, 0, st, a);
   } else if (direct && tiles >= 1024 && a.K >= 512 && a.N >= 256) {
     nt_tiles<T, 256, 256, 2, 4, 2, 2, 1>(a, direct, st);
   } else {
@@ -1126,9 +1177,10 @@ void nt_launch(GemmArgs a, hipStream_t st) {
 template <typename T>
 void tn_launch(const TnArgs &a, bool da, bool db, hipStream_t st) {
   const dim3 g(a.tiles_n * a.tiles_k * a.slices), b(kThreads);
-  if (da && db) hipLaunchKernelGGL((tn_kernel<T, true, true>), g, b, 0, st, a);
-  else if (da) hipLaunchKernelGGL((tn_kernel<T, true, false>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((tn_kernel<T, false, false>), g, b, 0, st, a);
+  if (a.N < 8 || a.K < 8) hipLaunchKernelGGL((tn_kernel<T, kElems, kElems>), g, b, 0, st, a);
+  else if (da && db) hipLaunchKernelGGL((tn_kernel<T, kWords, kWords>), g, b, 0, st, a);
+  else if (da) hipLaunchKernelGGL((tn_kernel<T, kWords, kRegs>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((tn_kernel<T, kRegs, kRegs>), g, b, 0, st, a);
 }
 
 #define SHD_DISPATCH_16(DTYPE, ...)                         \
@@ -1237,7 +1289,7 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
     SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, da, x_words, st);
                     else if (bits_dw) tn_narrow_launch<T, true>(n, st);
                     else tn_narrow_launch<T, false>(n, st);
-                    if (joined) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)((joined + 255) / 256)), dim3(256), 0, st, a.part, a.part_b, p.slices, N, K,
+                    if (joined) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)((joined + 63) / 64)), dim3(256), 0, st, a.part, a.part_b, p.slices, N, K,
                                                    (T *)d_dw, lddw, d_db, db_f32));
     SHD_HIP(hipGetLastError());
   }

@@ -302,7 +302,7 @@ def _lin_check(x, W, b, act, res, dy):
 
 
 _SIZES = [(1, 1, 1), (1, 64, 8), (3, 5, 7), (17, 31, 33), (128, 128, 64), (129, 257, 65), (256, 256, 256), (1000, 47, 500), (300, 172, 602), (2049, 96, 100),
-          (63, 1000, 513), (4096, 8, 24), (130, 384, 1000), (5, 2000, 72)]
+          (63, 1000, 513), (4096, 8, 24), (130, 384, 1000), (5, 2000, 72), (9000, 5, 600), (9000, 600, 5), (8300, 9, 15)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
