@@ -508,43 +508,69 @@ __global__ void __launch_bounds__(WM * WN * 64, OCC) nt_kernel(GemmArgs a) {
 
 // Few output tiles: 32 x 32 tiles, the contraction cut over the workgroup's eight wavefronts (step 16 w, 16 (w + 8), ...), their
 // products joined in LDS in wavefront order.  Operands go from memory to the product's registers: every word is used once.
-template <typename T, Via VIA>
-__global__ void __launch_bounds__(512) nt_few_kernel(GemmArgs a) {
+// COLS (dx = dz W): B is given as [K, N]; A is dy and its words become dz = dy act'(z) on the way (kept_act 0: as they are).
+struct FewArgs {
+  GemmArgs g;
+  const char *kept;
+  int kept_act;
+};
+template <typename T, Via VIA, bool COLS>
+__global__ void __launch_bounds__(512) nt_few_kernel(FewArgs f) {
+  const GemmArgs &a = f.g;
   typedef typename Frag<T>::v8 v8;
   constexpr int kPitch = 36;
   __shared__ __attribute__((aligned(16))) float part[8][32 * kPitch];
   const uint32_t tm = blockIdx.x % a.tiles_m, tn = blockIdx.x / a.tiles_m, m0 = tm * 32, n0 = tn * 32;
   const uint32_t lane = lane_id(), wave = wave_id(), r = lane & 31;
-  const T *pa = static_cast<const T *>(a.A) + (int64_t)min(m0 + r, a.M - 1) * a.lda;
-  const T *pb = static_cast<const T *>(a.B) + (int64_t)min(n0 + r, a.N - 1) * a.ldb;
+  const uint32_t row_a = min(m0 + r, a.M - 1), row_b = min(n0 + r, a.N - 1);
+  const T *pa = static_cast<const T *>(a.A) + (int64_t)row_a * a.lda;
+  const T *pb = static_cast<const T *>(a.B) + (COLS ? (int64_t)row_b : (int64_t)row_b * a.ldb);
+  const char *pk = f.kept + (uint64_t)row_a * kept_pitch(f.kept_act, a.K);
   f32x16 acc;
 #pragma unroll
   for (int e = 0; e < 16; e++) acc[e] = 0.f;
   constexpr int U = 4;                       // steps whose loads are in flight together
   for (uint32_t k0 = wave * 16; k0 < a.K; k0 += 8 * 16 * U) {
-    uint4 wa[U], wb[U];
+    uint4 wa[U], wb[U], wz[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
-      if (VIA == kWords) {
-        const bool in = k < a.K;
-        wa[u] = in ? *reinterpret_cast<const uint4 *>(pa + k) : make_uint4(0, 0, 0, 0);
-        wb[u] = in ? *reinterpret_cast<const uint4 *>(pb + k) : make_uint4(0, 0, 0, 0);
+      if (VIA == kWords) wa[u] = k < a.K ? *reinterpret_cast<const uint4 *>(pa + k) : make_uint4(0, 0, 0, 0);
+      else if (VIA == kRegs) wa[u] = fetch_word(pa, k, a.K);
+      else wa[u] = load_elems(pa, k, a.K);
+      if (COLS) {
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = pb[(int64_t)min(k + j, a.K - 1) * a.ldb];
+        __builtin_memcpy(&wb[u], e, 16);
+        wz[u] = make_uint4(0, 0, 0, 0);
+        if (f.kept_act && k < a.K) {
+          if (keeps_bits(f.kept_act)) wz[u].x = (uint8_t)pk[k / 8];
+          else wz[u] = *reinterpret_cast<const uint4 *>(pk + k * 2);
+        }
+      } else if (VIA == kWords) {
+        wb[u] = k < a.K ? *reinterpret_cast<const uint4 *>(pb + k) : make_uint4(0, 0, 0, 0);
       } else if (VIA == kRegs) {
-        wa[u] = fetch_word(pa, k, a.K);
         wb[u] = fetch_word(pb, k, a.K);
       } else {
-        wa[u] = load_elems(pa, k, a.K);
         wb[u] = load_elems(pb, k, a.K);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
+      const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
       v8 fa, fb;
       if (VIA == kRegs) {
-        const uint32_t k = k0 + u * 128 + (lane >> 5) * 8;
         wa[u] = settle_word(wa[u], k, a.K);
-        wb[u] = settle_word(wb[u], k, a.K);
+        if (!COLS) wb[u] = settle_word(wb[u], k, a.K);
+      }
+      if (COLS) {
+        if (f.kept_act) wa[u] = dz_word<T>(f.kept_act, wa[u], wz[u]);
+        T e[8];
+        __builtin_memcpy(e, &wb[u], 16);
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = k + j < a.K ? e[j] : (T)0.f;
+        __builtin_memcpy(&wb[u], e, 16);
       }
       __builtin_memcpy(&fa, &wa[u], 16);
       __builtin_memcpy(&fb, &wb[u], 16);
@@ -1020,6 +1046,76 @@ __global__ void __launch_bounds__(NB * KB * 64, 2) tn_narrow_kernel(TnNarrowArgs
     }
 }
 
+// dz^T x over few rows: 32 x 32 tiles of dW, the rows cut over the workgroup's eight wavefronts (16 at a time) and joined in LDS in
+// wavefront order; dz is formed element by element from dy and what was kept.  One launch, no scratch; db from the tiles of the first
+// 32 columns of x.
+struct TnFewArgs {
+  TnArgs t;
+  const char *kept;
+  int kept_act;                              // 0: A is dz
+  void *db;
+  int db_f32;
+};
+template <typename T>
+__global__ void __launch_bounds__(512) tn_few_kernel(TnFewArgs f) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int kPitch = 33;
+  __shared__ float part[8][32 * kPitch], part_b[8][64];
+  const TnArgs &a = f.t;
+  const uint32_t tn = blockIdx.x / a.tiles_k, tk = blockIdx.x % a.tiles_k, n0 = tn * 32, k0 = tk * 32;
+  const uint32_t lane = lane_id(), wave = wave_id(), c = lane & 31;
+  const uint32_t n = min(n0 + c, a.N - 1), k = min(k0 + c, a.K - 1);
+  const uint64_t pitch = kept_pitch(f.kept_act, a.N);
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; e++) acc[e] = 0.f;
+  float sum = 0.f;
+  for (uint32_t m0 = wave * 16 + (lane >> 5) * 8; m0 - (lane >> 5) * 8 < a.M; m0 += 128) {
+    T ea[8], eb[8];
+    float slope[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {            // (rows past the end repeat the last and are cleared below)
+      const uint32_t m = min(m0 + j, a.M - 1);
+      ea[j] = static_cast<const T *>(a.A)[(int64_t)m * a.lda + n];
+      eb[j] = static_cast<const T *>(a.B)[(int64_t)m * a.ldb + k];
+      slope[j] = !f.kept_act ? 0.f : keeps_bits(f.kept_act) ? (float)((uint8_t)f.kept[m * pitch + n / 8] >> (n & 7) & 1u)
+                                                            : (float)*reinterpret_cast<const f16_t *>(f.kept + m * pitch + n * 2);
+    }
+    v8 fa, fb;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float v = (float)ea[j];
+      if (f.kept_act) {
+        const float s = keeps_bits(f.kept_act) ? (slope[j] != 0.f ? 1.f : f.kept_act == 4 ? 0.2f : 0.f) : slope16(f.kept_act, slope[j]);
+        v = v == 0.f || s == 0.f ? 0.f : v * s;
+      }
+      const bool in = m0 + j < a.M;
+      fa[j] = in ? (T)v : (T)0.f;
+      fb[j] = in ? eb[j] : (T)0.f;
+      sum += (float)fa[j];
+    }
+    acc = mma(fa, fb, acc);                  // rows: n, columns (lanes): k
+  }
+#pragma unroll
+  for (int e = 0; e < 16; e++) part[wave][((e >> 2) * 8 + (lane >> 5) * 4 + (e & 3)) * kPitch + c] = acc[e];
+  part_b[wave][lane] = sum;
+  __syncthreads();
+  for (uint32_t o = threadIdx.x; o < 1024; o += 512) {
+    const uint32_t r = o >> 5, q = o & 31;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) t += part[w][r * kPitch + q];
+    if (n0 + r < a.N && k0 + q < a.K) static_cast<T *>(a.C)[(int64_t)(n0 + r) * a.ldc + k0 + q] = (T)t;
+  }
+  if (f.db && tk == 0 && threadIdx.x < 32 && n0 + threadIdx.x < a.N) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) t += part_b[w][threadIdx.x] + part_b[w][32 + threadIdx.x];
+    if (f.db_f32) static_cast<float *>(f.db)[n0 + threadIdx.x] = t;
+    else static_cast<T *>(f.db)[n0 + threadIdx.x] = (T)t;
+  }
+}
+
 // Sums of the slices: 64 outputs per workgroup, each of its four wavefronts every fourth slice, joined in wavefront order (always the
 // same order).  The first N K outputs are dW (part null: it is written already), N more db (part_b null: not wanted).
 template <typename T>
@@ -1106,6 +1202,10 @@ BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   return p;
 }
 
+// dz^T x in one launch of 32 x 32 tiles: 256 rows of 256 x 256 take 8 us so and 17 in slices of 128 x 128 tiles (dz, product, join),
+// 1024 rows 24 and 18
+bool few_rows(uint32_t M, uint32_t N, uint32_t K) { return M <= 512 && (uint64_t)((N + 31) / 32) * ((K + 31) / 32) <= 1024; }
+
 bool dtype16(int d) { return d == SL_BF16 || d == SL_F16; }
 
 template <typename T, int BM_, int BN_, int WM, int WN, int ST, int OCC, int PERCU>
@@ -1146,6 +1246,17 @@ void tn_narrow_launch(const TnNarrowArgs &n, hipStream_t st) {
   }
 }
 
+inline uint64_t tiles128(uint32_t M, uint32_t N) { return (uint64_t)((M + 127) / 128) * ((N + 127) / 128); }
+
+template <typename T, bool COLS>
+void few_launch(FewArgs f, bool words, hipStream_t st) {
+  f.g.tiles_m = (f.g.M + 31) / 32; f.g.tiles_n = (f.g.N + 31) / 32;
+  const dim3 g(f.g.tiles_m * f.g.tiles_n), b(512);
+  if (words) hipLaunchKernelGGL((nt_few_kernel<T, kWords, COLS>), g, b, 0, st, f);
+  else if (f.g.K >= 8) hipLaunchKernelGGL((nt_few_kernel<T, kRegs, COLS>), g, b, 0, st, f);
+  else hipLaunchKernelGGL((nt_few_kernel<T, kElems, COLS>), g, b, 0, st, f);
+}
+
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);
@@ -1156,17 +1267,15 @@ void nt_launch(GemmArgs a, hipStream_t st) {
     else narrow_launch<T, 0>(n, st);
     return;
   }
-  const uint64_t tiles = (uint64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
   // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches and contractions of less
   //  than eight are rare and take the other)
   // (fewer than 64 tiles of 128: 1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128 ones, twice the
   //  rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47)
+  const uint64_t tiles = tiles128(a.M, a.N);
   if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22) || a.K < 8) {
-    a.tiles_m = (a.M + 31) / 32; a.tiles_n = (a.N + 31) / 32;
-    const dim3 g(a.tiles_m * a.tiles_n), b(512);
-    if (direct) hipLaunchKernelGGL((nt_few_kernel<T, kWords>), g, b, 0, st, a);
-    else if (a.K >= 8) hipLaunchKernelGGL((nt_few_kernel<T, kRegs>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((nt_few_kernel<T, kElems>), g, b, 0, st, a);
+    FewArgs f = {};
+    f.g = a;
+    few_launch<T, false>(f, direct, st);
   } else if (direct && tiles >= 1024 && a.K >= 512 && a.N >= 256) {
     nt_tiles<T, 256, 256, 2, 4, 2, 2, 1>(a, direct, st);
   } else {
@@ -1242,9 +1351,10 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
   const bool dy_words = rows_of_words(d_dy, lddy, N, SL_BF16), x_words = rows_of_words(d_x, ldx, K, SL_BF16), shape = narrow_shape(M, N, K);
   const bool narrow_dx = d_dx && shape && dy_words, narrow_dw = want_w && shape && x_words && (act || dy_words);
   const bool bits_dw = narrow_dw && keeps_bits(act) && dy_words;       // (dz^T x masks dy itself)
+  const bool few_dx = d_dx && M && !narrow_dx && tiles128(M, K) < 64, few_dw = want_w && M && !narrow_dw && few_rows(M, N, K);
   const BwdPlan p = plan_bwd(act, M, N, K, narrow_dw);
   char *ws = static_cast<char *>(d_scratch);
-  const bool need_dz = act && M && ((d_dx && !narrow_dx) || (want_w && !bits_dw));
+  const bool need_dz = act && M && ((d_dx && !narrow_dx && !few_dx) || (want_w && !bits_dw && !few_dw));
   const int64_t ldp = (int64_t)up(N, 8);
   const void *dz = need_dz ? ws + p.dz : d_dy;
   const int64_t lddz = need_dz ? ldp : lddy;
@@ -1265,6 +1375,13 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
                     else if (keeps_bits(act)) narrow_launch<T, 3>(n, st);
                     else narrow_launch<T, 2>(n, st));
     SHD_HIP(hipGetLastError());
+  } else if (few_dx) {
+    FewArgs f = {};
+    f.g.A = dz; f.g.lda = lddz; f.g.B = d_w; f.g.ldb = ldw; f.g.M = M; f.g.N = K; f.g.K = N; f.g.C = d_dx; f.g.ldc = lddx;
+    f.kept = static_cast<const char *>(d_kept); f.kept_act = need_dz ? 0 : act;
+    SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, few_launch<T, true>(f, rows_of_words(dz, lddz, N, SL_BF16), st));
+    SHD_HIP(hipGetLastError());
   } else if (d_dx && M) {
     GemmArgs a = {};
     a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldp; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
@@ -1275,7 +1392,15 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
                     nt_launch<T>(a, st));
     SHD_HIP(hipGetLastError());
   }
-  if (want_w) {
+  if (few_dw) {
+    TnFewArgs f = {};
+    TnArgs &a = f.t;
+    a.A = dz; a.lda = lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + 31) / 32; a.tiles_k = (K + 31) / 32; a.C = d_dw; a.ldc = lddw;
+    f.kept = static_cast<const char *>(d_kept); f.kept_act = need_dz ? 0 : act; f.db = d_db; f.db_f32 = db_f32;
+    SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dw_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((tn_few_kernel<T>), dim3(a.tiles_n * a.tiles_k), dim3(512), 0, st, f));
+    SHD_HIP(hipGetLastError());
+  } else if (want_w) {
     TnNarrowArgs n = {};
     TnArgs &a = n.t;
     a.A = bits_dw ? d_dy : dz; a.lda = bits_dw ? lddy : lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + BN - 1) / BN;
