@@ -164,6 +164,7 @@ extern "C" int sl_dropout(int dtype, const void *d_x, int64_t ldx, const void *d
                           uint64_t seed, const int64_t *d_seed, void *d_y, int64_t ldy, void *stream) {
   if (!elem_dtype_ok(dtype)) return set_error(SG_ERR_INVALID, "sl_dropout: type %d", dtype);
   if (!(p >= 0.f && p < 1.f)) return set_error(SG_ERR_INVALID, "sl_dropout: probability %g (0 <= p < 1)", (double)p);
+  if (F > 0x7FFFFFFFu) return set_error(SG_ERR_INVALID, "sl_dropout: rows of %u elements", F);
   if (n == 0 || F == 0) return SG_OK;
   if (!d_x || !d_y || ldx < (int64_t)F || ldy < (int64_t)F || (d_res && ldr < (int64_t)F)) return set_error(SG_ERR_INVALID, "sl_dropout: operands");
   hipStream_t st = (hipStream_t)stream;

@@ -616,7 +616,7 @@ extern "C" int sl_label_logprobs_fwd(int dtype, const void *d_x, int64_t ldx, co
       a.part = static_cast<float *>(d_scratch);
       a.part_top = reinterpret_cast<int2 *>(a.part + (size_t)n * a.splits * 4);
     }
-    if ((uint64_t)n * a.splits > 0x7FFFFFFFull) return set_error(SG_ERR_INVALID, "sl_label_logprobs_fwd: grid");
+    if ((uint64_t)n * a.splits > 0xFFFFFFull) return set_error(SG_ERR_INVALID, "sl_label_logprobs_fwd: %u rows of %u classes", n, C);
     SHD_DISPATCH_ELEM(dtype, stream_launch<T>(a, st));
   }
   SHD_HIP(hipGetLastError());

@@ -2,8 +2,10 @@
 // in its epilogue, and its gradients:
 //     z = x W^T + b,   y = act(z) + res,   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum_rows dz
 //
-// Three kernels for x W^T and dz W (the weight transposed once per call, it is small): 256 x 256 tiles for large products, 128 x 128
-// for the others, 32 x 32 with the contraction cut over wavefronts where there are few tiles; one for dz^T x.
+// x W^T and dz W: 256 x 256 tiles for large products, 128 x 128 for the others, 32 x 32 with the contraction cut over wavefronts where
+// there are few tiles (nt_launch has the rule), and for tall, narrow operands a kernel that keeps the weight in registers.  dz W reads
+// the weight by columns in the last two, and transposed (once per call, it is small) in the others.  dz^T x: 128 x 128 tiles over row
+// slices, all of dW at once for narrow operands, 32 x 32 tiles in one launch for few rows.
 // Tiles are staged in LDS 64 steps of the contraction at a time -- 128 bytes of every row: with half lines (32 steps) every line
 // crossed to the CU twice, 338 instead of 314 us at 32768 x 1024 x 4096 -- and multiplied on 32x32x16 products formed as W x^T: a lane then
 // holds four neighbouring output COLUMNS of a row.
@@ -1162,7 +1164,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, cons
 template <typename T>
 __global__ void __launch_bounds__(256) transpose_kernel(const T *W, int64_t ldw, uint32_t N, uint32_t K, T *out, int64_t ld) {
   __shared__ T tile[32][33];
-  const uint32_t n0 = blockIdx.y * 32, k0 = blockIdx.x * 32, c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const uint32_t across = (K + 31) / 32, n0 = blockIdx.x / across * 32, k0 = blockIdx.x % across * 32, c = threadIdx.x & 31, r = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
     tile[r + i][c] = n0 + r + i < N && k0 + c < K ? W[(int64_t)(n0 + r + i) * ldw + k0 + c] : (T)0.f;
@@ -1184,9 +1186,9 @@ struct BwdPlan {
 BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   BwdPlan p;
   p.narrow = narrow;
-  const uint32_t tiles = ((N + BN - 1) / BN) * ((K + BM - 1) / BM);
+  const uint64_t tiles = (uint64_t)((N + BN - 1) / BN) * ((K + BM - 1) / BM);
   // row slices of dz^T x: one workgroup per CU, at least four stages each
-  uint32_t s = narrow ? 256 : 256 / tiles;
+  uint32_t s = narrow || tiles == 0 ? 256 : (uint32_t)(256 / tiles);
   const uint32_t most = (M + 4 * BK - 1) / (4 * BK);
   s = s < 1 ? 1 : s;
   s = s > most ? most : s;
@@ -1257,6 +1259,15 @@ void few_launch(FewArgs f, bool words, hipStream_t st) {
   else hipLaunchKernelGGL((nt_few_kernel<T, kElems, COLS>), g, b, 0, st, f);
 }
 
+// x W^T in 32 x 32 tiles: fewer than 64 tiles of 128 (1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128
+// ones, twice the rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47); and what the tile kernel does not
+// hold: its offsets (256 rows of a pitch below 2^22 elements stay below 2^31 bytes) and contractions of less than eight, both rare
+bool takes_few(uint32_t M, uint32_t N, uint32_t K, int64_t lda, int64_t ldb) {
+  return tiles128(M, N) < 64 || lda >= (1 << 22) || ldb >= (1 << 22) || K < 8;
+}
+// its grid: a launch has fewer than 2^32 threads
+bool few_fits(uint32_t M, uint32_t N) { return (((uint64_t)M + 31) / 32) * (((uint64_t)N + 31) / 32) < 1u << 23; }
+
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);
@@ -1267,12 +1278,8 @@ void nt_launch(GemmArgs a, hipStream_t st) {
     else narrow_launch<T, 0>(n, st);
     return;
   }
-  // (the tile kernel's offsets: 256 rows of a pitch below 2^22 elements stay below 2^31 bytes; wider pitches and contractions of less
-  //  than eight are rare and take the other)
-  // (fewer than 64 tiles of 128: 1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128 ones, twice the
-  //  rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47)
   const uint64_t tiles = tiles128(a.M, a.N);
-  if (tiles < 64 || a.lda >= (1 << 22) || a.ldb >= (1 << 22) || a.K < 8) {
+  if (takes_few(a.M, a.N, a.K, a.lda, a.ldb)) {
     FewArgs f = {};
     f.g = a;
     few_launch<T, false>(f, direct, st);
@@ -1296,7 +1303,7 @@ void tn_launch(const TnArgs &a, bool da, bool db, hipStream_t st) {
   if ((DTYPE) == SL_BF16) { using T = bf16_t; __VA_ARGS__; }\
   else { using T = f16_t; __VA_ARGS__; }
 
-constexpr uint64_t kMaxTiles = 0x7FFFFFFFull;
+constexpr uint64_t kMaxTiles = 0xFFFFFFull;   // of 256 threads each
 
 int check_sizes(const char *who, int dtype, int act, uint32_t M, uint32_t N, uint32_t K) {
   if (!dtype16(dtype)) return set_error(SG_ERR_INVALID, "%s: type %d (bf16 or fp16 operands)", who, dtype);
@@ -1318,6 +1325,7 @@ extern "C" int sl_linear16_fwd(int dtype, const void *d_x, int64_t ldx, const vo
   if (!d_x || !d_w || !d_y || ldx < (int64_t)K || ldw < (int64_t)K || ldy < (int64_t)N || (d_res && ldr < (int64_t)N) ||
       (d_kept && (reinterpret_cast<uintptr_t>(d_kept) & 15)))
     return set_error(SG_ERR_INVALID, "sl_linear16_fwd: operands");
+  if (takes_few(M, N, K, ldx, ldw) && !few_fits(M, N)) return set_error(SG_ERR_INVALID, "sl_linear16_fwd: too many tiles");
   hipStream_t st = (hipStream_t)stream;
   GemmArgs a = {};
   a.A = d_x; a.lda = ldx; a.B = d_w; a.ldb = ldw; a.M = M; a.N = N; a.K = K; a.bias = d_bias; a.bias_f32 = bias_f32; a.res = d_res; a.ldr = ldr;
@@ -1347,6 +1355,9 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
              (d_dx && (!d_w || ldw < (int64_t)K || lddx < (int64_t)K)) || (want_w && (!d_x || ldx < (int64_t)K)))))
     return set_error(SG_ERR_INVALID, "sl_linear16_bwd: operands");
   if (d_db && !d_dw) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: db comes with dW");
+  // (dx: dz's pitch is N or less than eight more; dy's own can be wider)
+  if (d_dx && takes_few(M, K, act ? (uint32_t)up(N, 8) : N, act ? (int64_t)up(N, 8) : lddy, (int64_t)up(N, 8)) && !few_fits(M, K)) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: too many tiles");
+  if (((uint64_t)(K + 31) / 32) * (((uint64_t)N + 31) / 32) > kMaxTiles) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: weight of %u x %u", N, K);
   hipStream_t st = (hipStream_t)stream;
   const bool dy_words = rows_of_words(d_dy, lddy, N, SL_BF16), x_words = rows_of_words(d_x, ldx, K, SL_BF16), shape = narrow_shape(M, N, K);
   const bool narrow_dx = d_dx && shape && dy_words, narrow_dw = want_w && shape && x_words && (act || dy_words);
@@ -1387,7 +1398,7 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
     a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldp; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
     a.K = act ? (uint32_t)ldp : N;           // (dz of an activation has zero pad columns, as W^T has: whole words)
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((transpose_kernel<T>), dim3((K + 31) / 32, (uint32_t)((ldp + 31) / 32)), dim3(256), 0, st, (const T *)d_w, ldw, N, K,
+    SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((transpose_kernel<T>), dim3((K + 31) / 32 * (uint32_t)((ldp + 31) / 32)), dim3(256), 0, st, (const T *)d_w, ldw, N, K,
                                               (T *)(ws + p.wt), ldp);
                     nt_launch<T>(a, st));
     SHD_HIP(hipGetLastError());

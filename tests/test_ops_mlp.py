@@ -102,6 +102,12 @@ P = (C.addressof(_BUF) + 255) // 256 * 256          # a host address: the calls 
     ("sl_label_logprobs_fwd", (1, P, 131072, P, 1, 1, 131072, 0, P, P, P, None, None, None, None)),   # a split row without scratch
     ("sl_label_logprobs_bwd", (1, P, 8, P, 1, 1, 8, 0, P, P, None, None, None, None, None, 8, None)),  # no dx
     ("sl_label_logprobs_bwd", (1, P, 8, P, 1, 1, 8, 2, P, P, None, None, None, P, P, 8, None)),        # dtop without indices
+    ("sl_dropout", (1, P, 1 << 32, None, 0, 1, (1 << 31) + 8, 0.5, 1, None, P, 1 << 32, None)),        # columns are counted in 32 bits
+    ("sl_linear16_fwd", (1, P, 4, P, 4, None, 0, None, 0, (1 << 31) - 1, 1, 4, 0, P, 1, None, None)),   # a launch of 2^32 threads and more
+    ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, (1 << 31) - 1, 1 << 24, 8, 0, P, 1 << 24, None, None)),
+    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 2, None, (1 << 31) - 1, 2, 8, 0, P, 8, None, 0, None, 0, P, None)),
+    ("sl_linear16_bwd", (1, P, 1 << 24, P, 1 << 24, P, 1 << 24, None, 1, 1 << 24, 1 << 24, 0, P, 1 << 24, None, 0, None, 0, P, None)),
+    ("sl_label_logprobs_fwd", (1, P, 2000, P, 1, 1 << 25, 2000, 0, P, P, P, None, None, None, None)),
 ])
 def test_c_entries_refuse(name, args):
     lib = _lib.load()
@@ -119,3 +125,5 @@ def test_sizes_of_scratch():
     assert lib.sl_label_logprobs_scratch_bytes(1, 1, 131072, 10) > 0         # one row: split
     assert lib.sl_linear16_bwd_scratch_bytes(1, 0, 8, 8) > 0
     assert lib.sl_linear16_kept_bytes(0, 10, 64) == 0 and lib.sl_linear16_kept_bytes(1, 10, 129) == 320 and lib.sl_linear16_kept_bytes(5, 10, 129) == 10 * 136 * 2
+    # the largest weight of the documented range (2^34 tiles): a size, not a division by their number in 32 bits
+    assert lib.sl_linear16_bwd_scratch_bytes(0, 1000, 1 << 24, 1 << 24) > 1 << 48

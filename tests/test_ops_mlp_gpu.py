@@ -625,6 +625,91 @@ def test_rows_behind_the_last_stay_as_they_were():
                 assert not (rows[:n, :width] == 77).all(), name
 
 
+@pytest.mark.parametrize("M,N,K,act", [
+    (16411, 256, 256, 1), (16411, 128, 72, 5), (16387, 72, 136, 4), (16393, 40, 16, 0),      # tall, narrow: whole words
+    (1111, 1100, 264, 2), (1111, 1100, 263, 1),                                             # 128 x 128 tiles, words and any rows
+    (4100, 4200, 520, 6),                                                                   # 256 x 256 tiles
+    (530, 300, 100, 1), (512, 300, 101, 5),                                                 # rows on both sides of the few-row gradient
+])
+def test_linear16_writes_its_own_elements_only(M, N, K, act):
+    """Outputs in pitched buffers, what is kept and the scratch in buffers of the stated sizes: all that lies behind stays as it was."""
+    from shadow_gnn_amd import _lib
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    g = _gen(57)
+    x, W, r = _randn(g, M, K, dtype=BF16), _randn(g, N, K, dtype=BF16, scale=K ** -0.5), _randn(g, M, N, dtype=BF16)
+    kb, sb = lib.sl_linear16_kept_bytes(act, M, N), lib.sl_linear16_bwd_scratch_bytes(act, M, N, K)
+    kept = torch.full((kb + 4096,), 0x5A, dtype=torch.uint8, device=DEV)
+    ws = torch.full((sb + 4096,), 0x5A, dtype=torch.uint8, device=DEV)
+
+    def rows(n, width):
+        return torch.full((n + 3, width + 16), 77.0, dtype=BF16, device=DEV)
+
+    y, dx, dw, db = rows(M, N), rows(M, K), rows(N, K), torch.full((N + 64,), 77.0, device=DEV)
+    assert lib.sl_linear16_fwd(1, x.data_ptr(), K, W.data_ptr(), K, None, 0, r.data_ptr(), N, M, N, K, act, y.data_ptr(), N + 16, kept.data_ptr() if act else None, st) == 0
+    assert lib.sl_linear16_bwd(1, x.data_ptr(), K, W.data_ptr(), K, r.data_ptr(), N, kept.data_ptr() if act else None, M, N, K, act, dx.data_ptr(), K + 16,
+                               dw.data_ptr(), K + 16, db.data_ptr(), 1, ws.data_ptr(), st) == 0
+    torch.cuda.synchronize()
+    assert (kept[kb:] == 0x5A).all() and (ws[sb:] == 0x5A).all() and (db[N:] == 77).all()
+    for t, n, width in ((y, M, N), (dx, M, K), (dw, N, K)):
+        assert (t[:, width:] == 77).all() and (t[n:] == 77).all() and (t[:n, :width] != 77).any(1).all()
+
+
+def test_gradients_are_differentiable_once():
+    """create_graph gives the same gradients; a second backward pass through them is an error, not zeros."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(58)
+    x, W, s = _randn(g, 64, 64, dtype=BF16).requires_grad_(True), _randn(g, 64, 64, dtype=BF16, scale=0.1).requires_grad_(True), _randn(g, 64).requires_grad_(True)
+    label = torch.randint(0, 64, (64,), device=DEV, generator=g)
+    dy = _randn(g, 64, 64, dtype=BF16).requires_grad_(True)
+    for f in (lambda: ops_mlp.layer_norm(x, s, s), lambda: ops_mlp.dropout(x, 0.5, 3), lambda: ops_mlp.linear_act(x, W, act="gelu")):
+        plain = torch.autograd.grad(f(), x, dy.detach())[0]
+        twice = torch.autograd.grad(f(), x, dy, create_graph=True)[0]
+        assert torch.equal(plain, twice.detach())
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(twice.float().sum(), dy)
+    first = torch.autograd.grad(ops_mlp.label_logprobs(x, label).entropy.sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        first.float().sum().backward()
+
+
+def test_one_tensor_in_several_places():
+    """Scale and offset, x and residual, x and weight may be one tensor: its gradient is the sum of both places'."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(59)
+    x, s, dy = _randn(g, 128, 128, dtype=BF16), _randn(g, 128), _randn(g, 128, 128, dtype=BF16)
+
+    def both(f, t):
+        one = t.clone().requires_grad_(True)
+        a, b = t.clone().requires_grad_(True), t.clone().requires_grad_(True)
+        y, z = f(one, one), f(a, b)
+        assert torch.equal(y, z)
+        got, want = torch.autograd.grad(y, one, dy)[0], torch.autograd.grad(z, [a, b], dy)
+        assert torch.equal(got, want[0] + want[1])
+
+    both(lambda a, b: ops_mlp.layer_norm(x, a, b), s)
+    both(lambda a, b: ops_mlp.dropout(a, 0.3, 4, residual=b), x)
+    both(lambda a, b: ops_mlp.linear_act(a, x, act="relu", residual=b), x)
+    both(lambda a, b: ops_mlp.linear_act(a, b, act="silu"), x)
+
+
+def test_tensors_changed_before_the_backward_pass_are_noticed():
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(60)
+    W, label = _randn(g, 64, 64, dtype=BF16).requires_grad_(True), torch.zeros(64, dtype=torch.int64, device=DEV)
+    seed = torch.tensor([5], device=DEV)
+    x = _randn(g, 64, 64, dtype=BF16)
+
+    def changed(f, t, leaf):
+        y = f()
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), leaf)
+
+    changed(lambda: ops_mlp.linear_act(x, W), x, W)
+    changed(lambda: ops_mlp.dropout(W, 0.5, seed), seed, W)
+    changed(lambda: ops_mlp.label_logprobs(W, label).logprob, label, W)
+
+
 def test_offsets_past_32_bits():
     """Rows 2^30 + 8 elements apart: the third begins past 2^31 elements."""
     from shadow_gnn_amd import ops, ops_mlp
