@@ -601,6 +601,106 @@ __global__ void __launch_bounds__(512) nt_few_kernel(FewArgs f) {
   finish8<T>(a, m, n, left, v, b, resw);
 }
 
+// dx = dz W of few outputs (N <= 64: a classifier's classes): B is W as it is, [K, N] here.  A wavefront keeps 64 columns of W in
+// registers and walks `per` tiles of 32 rows, a tile ahead of its loads; no barriers, no tile of A in LDS (it would be read once), no
+// transposed weight.  Wavefronts of one workgroup share rows.  Bound by the loads' latency at a few wavefronts per SIMD: dx of
+// 20011 x 64 -> 512 takes 12 us (4 of them the store) and 18 in transposed 128 x 128 tiles, 8192 x 40 -> 1024 10 and 14.
+template <typename T>
+__global__ void __launch_bounds__(256, 4) nt_short_kernel(GemmArgs a, uint32_t groups, uint32_t per) {
+  typedef typename Frag<T>::v8 v8;
+  constexpr int Q = 4;
+  __shared__ __attribute__((aligned(16))) float corners[4][16 * 64];
+  const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), item = blockIdx.x * 4 + wave, n0 = item % groups * 64;
+  const uint32_t tile0 = item / groups * per, tiles = (a.M + 31) / 32;
+  if (tile0 >= tiles) return;                // (whole wavefronts; no barrier follows)
+  const uint32_t tile1 = min(tiles, tile0 + per), kl = (lane >> 5) * 8;
+  uint4 wa[Q];
+  auto fetch = [&](uint32_t tile) {
+    const T *pa = static_cast<const T *>(a.A) + (int64_t)min(tile * 32 + (lane & 31), a.M - 1) * a.lda;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+      const uint32_t k = q * 16 + kl;
+      wa[q] = *reinterpret_cast<const uint4 *>(pa + (k < a.K ? k : 0));
+    }
+  };
+  v8 fb[2][Q];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {              // (32-bit offsets: the host keeps the pitch below 2^22 elements)
+    const uint32_t col = min(n0 + h * 32 + (lane & 31), a.N - 1);
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+      T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        e[j] = *reinterpret_cast<const T *>(static_cast<const char *>(a.B) + (min(q * 16 + kl + j, a.K - 1) * (uint32_t)a.ldb + col) * 2);
+      __builtin_memcpy(&fb[h][q], e, 16);
+    }
+  }
+  fetch(tile0);
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) fb[h][q][j] = q * 16 + kl + j < a.K ? fb[h][q][j] : (T)0.f;
+  float *mine = corners[wave];
+  const uint32_t er = lane >> 3, ec = lane & 7, n = n0 + ec * 8;
+  const int left = min(8, (int)a.N - (int)n);
+  uint32_t m = tile0 * 32 + er;              // this lane's next row
+  T *dst = static_cast<T *>(a.C) + (int64_t)m * a.ldc + n;
+  const int64_t step = 8 * a.ldc;
+  for (uint32_t tile = tile0; tile < tile1; tile++) {
+    v8 fa[Q];
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+      const uint32_t k = q * 16 + kl;
+      const uint4 w = k < a.K ? wa[q] : make_uint4(0, 0, 0, 0);
+      __builtin_memcpy(&fa[q], &w, 16);
+    }
+    if (tile + 1 < tile1) fetch(tile + 1);
+    f32x16 acc[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[h][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < Q; q++) acc[h] = mma(fb[h][q], fa[q], acc[h]);
+    }
+#pragma unroll
+    for (uint32_t half = 0; half < 2; half++) {               // 16 rows at a time through this wavefront's corner (word w of row r at w ^ r)
+      if (((lane >> 4) & 1) == half) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            *reinterpret_cast<float4 *>(mine + (lane & 15) * 64 + ((h * 8 + e * 2 + (lane >> 5)) ^ (lane & 15)) * 4) =
+                make_float4(acc[h][4 * e], acc[h][4 * e + 1], acc[h][4 * e + 2], acc[h][4 * e + 3]);
+      }
+      wave_order();
+#pragma unroll
+      for (uint32_t t = 0; t < 16; t += 8, m += 8, dst += step) {
+        const uint32_t r = t + er;
+        if (m < a.M && left > 0) {
+          T out[8];
+          float v[8];
+          *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2) ^ r) * 4);
+          *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(mine + r * 64 + ((ec * 2 + 1) ^ r) * 4);
+#pragma unroll
+          for (int e = 0; e < 8; e++) out[e] = (T)v[e];
+          if (left == 8) {
+            __builtin_memcpy(dst, out, 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 7; e++)
+              if (e < left) dst[e] = out[e];
+          }
+        }
+      }
+      wave_order();
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ tall, narrow products
 // N <= 256 and K <= 256 (the hidden widths of the graph models) over many rows are bound by memory: x, res and y cross it once.  The
 // weight stays in the registers of NWC wavefronts (32 output columns each) for the whole launch; four more wavefronts do nothing but
@@ -614,7 +714,7 @@ __global__ void __launch_bounds__(512) nt_few_kernel(FewArgs f) {
 // Bits kept by the forward pass are gathered in LDS and leave a tile later as whole words (as bytes they cost 25 us of 140).
 struct NarrowArgs {
   GemmArgs g;
-  int b_cols;                                // 1: B is given as [K, N] (pitch ldb)
+  uint32_t b_rows;                           // not 0: B is given as [b_rows, N] (pitch ldb); K may end inside a word of zeros past it
   const char *kept;                          // SIDE 2, 3: kept values of g.K columns
   int kept_act;
   void *dz;                                  // SIDE 2, 3: null, or where dz goes, pitch lddz
@@ -687,14 +787,14 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
   {
     // (loads without conditions, so that all are on their way together; K is a multiple of eight: a lane's eight exist or not)
     const uint32_t row = min(n0 + (lane & 31), a.N - 1);
-    if (n.b_cols) {
+    if (n.b_rows) {
 #pragma unroll
       for (int q = 0; q < KS; q++) {
         const uint32_t k = q * 16 + (lane >> 5) * 8;
-        const T *p = static_cast<const T *>(a.B) + (int64_t)(k < a.K ? k : 0) * a.ldb + row;
+        const T *p = static_cast<const T *>(a.B) + row;
         T e[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = p[j * a.ldb];
+        for (int j = 0; j < 8; j++) e[j] = p[(int64_t)min(k + j, n.b_rows - 1) * a.ldb];
         __builtin_memcpy(&fb[q], e, 16);
       }
     } else {
@@ -710,6 +810,10 @@ __global__ void __launch_bounds__((NWC + 4) * 64, 3) narrow_kernel(NarrowArgs n)
       if (q * 16 + (lane >> 5) * 8 >= a.K) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
         __builtin_memcpy(&fb[q], &zero, 16);
+      } else if (n.b_rows && q * 16 + (lane >> 5) * 8 + 8 > n.b_rows) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (q * 16 + (lane >> 5) * 8 + j >= n.b_rows) fb[q][j] = (T)0.f;
       }
   }
   float *mine = reinterpret_cast<float *>(lds + RS * kPlace) + wave * 512;             // 16 rows of 32 columns
@@ -1144,7 +1248,7 @@ __global__ void __launch_bounds__(256) tn_join_kernel(const float *__restrict__ 
 }
 
 // ------------------------------------------------------------------------------------------------ elementwise pieces
-// dz = dy act'(z) of every word; pad columns are zero
+// dz = dy act'(z) (an identity: dy) in rows of whole words, whose pad columns are zero
 template <typename T>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, const char *kept, T *dz, int64_t ld, uint32_t M, uint32_t N, int act) {
   const uint32_t words = (uint32_t)(ld / 8);
@@ -1154,9 +1258,9 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t lddy, cons
     const uint32_t w = (uint32_t)(i % words);
     const uint4 g = load_word(dy + (int64_t)m * lddy, w * 8, N);       // (zero past N)
     uint4 z = make_uint4(0, 0, 0, 0);
-    if (keeps_bits(act)) z.x = (uint8_t)kept[m * pitch + w];
-    else z = *reinterpret_cast<const uint4 *>(kept + m * pitch + w * 16);
-    *reinterpret_cast<uint4 *>(dz + (int64_t)m * ld + w * 8) = dz_word<T>(act, g, z);
+    if (act && keeps_bits(act)) z.x = (uint8_t)kept[m * pitch + w];
+    else if (act) z = *reinterpret_cast<const uint4 *>(kept + m * pitch + w * 16);
+    *reinterpret_cast<uint4 *>(dz + (int64_t)m * ld + w * 8) = act ? dz_word<T>(act, g, z) : g;
   }
 }
 
@@ -1174,8 +1278,11 @@ __global__ void __launch_bounds__(256) transpose_kernel(const T *W, int64_t ldw,
     if (k0 + r + i < K && n0 + c < ld) out[(int64_t)(k0 + r + i) * ld + n0 + c] = tile[c][r + i];
 }
 
-// the tall, narrow form: both widths up to 256 in whole words, and rows for a few 64-row tiles per CU
-bool narrow_shape(uint32_t M, uint32_t N, uint32_t K) { return N <= 256 && K <= 256 && N % 8 == 0 && K % 8 == 0 && M >= 16384; }
+// the tall, narrow form: widths up to 256, the contraction's in whole words (a gradient's dz is: pad columns), rows for two 32-row
+// tiles per CU
+bool narrow_shape(uint32_t M, uint32_t N, uint32_t K) { return N <= 256 && K <= 256 && K % 8 == 0 && M >= 16384; }
+// dx of so few outputs goes through nt_short_kernel (its wavefronts hold 64 steps of the contraction)
+constexpr uint32_t kShort = 64;
 
 struct BwdPlan {
   uint32_t slices, per;                      // of dz^T x
@@ -1183,7 +1290,7 @@ struct BwdPlan {
   uint64_t dz, wt, part, part_b, total;      // byte offsets in the scratch
 };
 
-BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
+BwdPlan plan_bwd(uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   BwdPlan p;
   p.narrow = narrow;
   const uint64_t tiles = (uint64_t)((N + BN - 1) / BN) * ((K + BM - 1) / BM);
@@ -1196,7 +1303,7 @@ BwdPlan plan_bwd(int act, uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   p.per = (uint32_t)up((M + s - 1) / s, BK);
   p.slices = M ? (M + p.per - 1) / p.per : 1;
   uint64_t at = 0;
-  p.dz = at; at += act ? up((uint64_t)M * up(N, 8) * 2, 256) : 0;
+  p.dz = at; at += up((uint64_t)M * up(N, 8) * 2, 256);
   p.wt = at; at += up((uint64_t)K * up(N, 8) * 2, 256);
   p.part = at; at += p.slices > 1 || narrow ? up((uint64_t)p.slices * N * K * 4, 256) : 0;
   p.part_b = at; at += up((uint64_t)p.slices * N * 4, 256);
@@ -1259,6 +1366,16 @@ void few_launch(FewArgs f, bool words, hipStream_t st) {
   else hipLaunchKernelGGL((nt_few_kernel<T, kElems, COLS>), g, b, 0, st, f);
 }
 
+template <typename T>
+void short_launch(const GemmArgs &a, hipStream_t st) {
+  const uint32_t groups = (a.N + 63) / 64, tiles = (a.M + 31) / 32;
+  // (as many tiles per wavefront as leave every SIMD two wavefronts, sixteen at most)
+  const uint64_t p = (uint64_t)tiles * groups / 2048;
+  const uint32_t per = p < 1 ? 1 : p > 16 ? 16 : (uint32_t)p;
+  const uint64_t items = ((uint64_t)tiles + per - 1) / per * groups;
+  hipLaunchKernelGGL((nt_short_kernel<T>), dim3((uint32_t)((items + 3) / 4)), dim3(256), 0, st, a, groups, per);
+}
+
 // x W^T in 32 x 32 tiles: fewer than 64 tiles of 128 (1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128
 // ones, twice the rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47); and what the tile kernel does not
 // hold: its offsets (256 rows of a pitch below 2^22 elements stay below 2^31 bytes) and contractions of less than eight, both rare
@@ -1271,7 +1388,9 @@ bool few_fits(uint32_t M, uint32_t N) { return (((uint64_t)M + 31) / 32) * (((ui
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);
-  if (direct && narrow_shape(a.M, a.N, a.K) && rows_of_words(a.res, a.ldr, a.N, SL_BF16)) {
+  // (what is kept of rows that are not whole words leaves this kernel slowly: 289127 x 256 -> 47 relu takes 66 us here and 57 in tiles,
+  //  without it 47 and 51, 128 -> 172 54 and 73)
+  if (direct && narrow_shape(a.M, a.N, a.K) && rows_of_words(a.res, a.ldr, a.N, SL_BF16) && (a.N % 8 == 0 || !a.kept)) {
     NarrowArgs n = {};
     n.g = a;
     if (a.res) narrow_launch<T, 1>(n, st);
@@ -1291,12 +1410,13 @@ void nt_launch(GemmArgs a, hipStream_t st) {
 }
 
 template <typename T>
-void tn_launch(const TnArgs &a, bool da, bool db, hipStream_t st) {
+void tn_launch(const TnArgs &a, bool dz_words, bool x_words, hipStream_t st) {
   const dim3 g(a.tiles_n * a.tiles_k * a.slices), b(kThreads);
-  if (a.N < 8 || a.K < 8) hipLaunchKernelGGL((tn_kernel<T, kElems, kElems>), g, b, 0, st, a);
-  else if (da && db) hipLaunchKernelGGL((tn_kernel<T, kWords, kWords>), g, b, 0, st, a);
-  else if (da) hipLaunchKernelGGL((tn_kernel<T, kWords, kRegs>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((tn_kernel<T, kRegs, kRegs>), g, b, 0, st, a);
+  if (!dz_words && a.K >= 8) hipLaunchKernelGGL((tn_kernel<T, kRegs, kRegs>), g, b, 0, st, a);       // (more than 64 columns)
+  else if (!dz_words) hipLaunchKernelGGL((tn_kernel<T, kRegs, kElems>), g, b, 0, st, a);
+  else if (x_words) hipLaunchKernelGGL((tn_kernel<T, kWords, kWords>), g, b, 0, st, a);
+  else if (a.K >= 8) hipLaunchKernelGGL((tn_kernel<T, kWords, kRegs>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((tn_kernel<T, kWords, kElems>), g, b, 0, st, a);
 }
 
 #define SHD_DISPATCH_16(DTYPE, ...)                         \
@@ -1341,7 +1461,8 @@ extern "C" size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N) {
 }
 
 extern "C" size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K) {
-  const uint64_t a = plan_bwd(act, M, N, K, false).total, b = narrow_shape(M, N, K) ? plan_bwd(act, M, N, K, true).total : 0;
+  (void)act;
+  const uint64_t a = plan_bwd(M, N, K, false).total, b = narrow_shape(M, N, K) ? plan_bwd(M, N, K, true).total : 0;
   return a > b ? a : b;
 }
 
@@ -1355,34 +1476,40 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
              (d_dx && (!d_w || ldw < (int64_t)K || lddx < (int64_t)K)) || (want_w && (!d_x || ldx < (int64_t)K)))))
     return set_error(SG_ERR_INVALID, "sl_linear16_bwd: operands");
   if (d_db && !d_dw) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: db comes with dW");
-  // (dx: dz's pitch is N or less than eight more; dy's own can be wider)
-  if (d_dx && takes_few(M, K, act ? (uint32_t)up(N, 8) : N, act ? (int64_t)up(N, 8) : lddy, (int64_t)up(N, 8)) && !few_fits(M, K)) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: too many tiles");
   if (((uint64_t)(K + 31) / 32) * (((uint64_t)N + 31) / 32) > kMaxTiles) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: weight of %u x %u", N, K);
   hipStream_t st = (hipStream_t)stream;
   const bool dy_words = rows_of_words(d_dy, lddy, N, SL_BF16), x_words = rows_of_words(d_x, ldx, K, SL_BF16), shape = narrow_shape(M, N, K);
-  const bool narrow_dx = d_dx && shape && dy_words, narrow_dw = want_w && shape && x_words && (act || dy_words);
+  // a dy of few columns whose rows are not whole words is first laid out in such rows: loads of unaligned rows, many times over, cost
+  // more (dx and dW of 20011 x 47 -> 500: 43 us so, 35 with the pass; 289127 x 47 -> 256: 152 and 117; 289127 x 172 -> 128: 120 and 133)
+  const bool pad = !act && !dy_words && N <= kShort, dz_words = act || pad || dy_words;
+  const bool narrow_dx = d_dx && shape && dz_words, narrow_dw = want_w && shape && x_words && dz_words;
   const bool bits_dw = narrow_dw && keeps_bits(act) && dy_words;       // (dz^T x masks dy itself)
-  const bool few_dx = d_dx && M && !narrow_dx && tiles128(M, K) < 64, few_dw = want_w && M && !narrow_dw && few_rows(M, N, K);
-  const BwdPlan p = plan_bwd(act, M, N, K, narrow_dw);
+  const bool few_dx = d_dx && M && !narrow_dx && tiles128(M, K) < 64, few_dw = want_w && M && !narrow_dw && few_rows(M, N, K),
+             short_dx = d_dx && M && !narrow_dx && !few_dx && N <= kShort && ldw < (1 << 22);
+  const BwdPlan p = plan_bwd(M, N, K, narrow_dw);
+  if (d_dx && !narrow_dx && !short_dx && takes_few(M, K, N, lddy, 0) && !few_fits(M, K)) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: too many tiles");
   char *ws = static_cast<char *>(d_scratch);
-  const bool need_dz = act && M && ((d_dx && !narrow_dx && !few_dx) || (want_w && !bits_dw && !few_dw));
+  // dz in memory, in rows of whole words, unless what reads it forms it itself
+  const bool need_dz = M && (act || pad) && ((d_dx && !few_dx && !(narrow_dx && dy_words)) || (want_w && !bits_dw && !few_dw));
   const int64_t ldp = (int64_t)up(N, 8);
   const void *dz = need_dz ? ws + p.dz : d_dy;
   const int64_t lddz = need_dz ? ldp : lddy;
   const double bytes_dx = 2.0 * ((double)M * K + (double)N * K + (double)M * N);
-  if (need_dz && !narrow_dx) {
+  if (need_dz && !(narrow_dx && dy_words)) {
     const uint64_t need = ((uint64_t)M * (ldp / 8) + 255) / 256;
     const dim3 g((uint32_t)(need < 8192 ? need : 8192)), b(256);
-    SHD_PROF_FMT(4.0 * M * N + (double)M * kept_pitch(act, N), 0, st, "linear16_dz_N%u", N);
+    SHD_PROF_FMT(4.0 * M * N + (act ? (double)M * kept_pitch(act, N) : 0), 0, st, "linear16_dz_N%u", N);
     SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((dz_kernel<T>), g, b, 0, st, (const T *)d_dy, lddy, (const char *)d_kept, (T *)(ws + p.dz), ldp, M, N, act));
     SHD_HIP(hipGetLastError());
   }
   if (narrow_dx) {
     NarrowArgs n = {};
-    n.g.A = d_dy; n.g.lda = lddy; n.g.B = d_w; n.g.ldb = ldw; n.g.M = M; n.g.N = K; n.g.K = N; n.g.C = d_dx; n.g.ldc = lddx;
-    n.b_cols = 1; n.kept = static_cast<const char *>(d_kept); n.kept_act = act; n.dz = need_dz ? ws + p.dz : nullptr; n.lddz = ldp;
-    SHD_PROF_FMT(bytes_dx + (act ? (double)M * kept_pitch(act, N) : 0), 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, if (!act) narrow_launch<T, 0>(n, st);
+    n.g.A = dy_words ? d_dy : dz; n.g.lda = dy_words ? lddy : lddz; n.g.B = d_w; n.g.ldb = ldw; n.g.M = M; n.g.N = K; n.g.K = (uint32_t)ldp; n.g.C = d_dx;
+    n.g.ldc = lddx; n.b_rows = N;
+    const int fused = dy_words ? act : 0;
+    n.kept = static_cast<const char *>(d_kept); n.kept_act = fused; n.dz = fused && need_dz ? ws + p.dz : nullptr; n.lddz = ldp;
+    SHD_PROF_FMT(bytes_dx + (fused ? (double)M * kept_pitch(act, N) : 0), 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, if (!fused) narrow_launch<T, 0>(n, st);
                     else if (keeps_bits(act)) narrow_launch<T, 3>(n, st);
                     else narrow_launch<T, 2>(n, st));
     SHD_HIP(hipGetLastError());
@@ -1393,10 +1520,16 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
     SHD_DISPATCH_16(dtype, few_launch<T, true>(f, rows_of_words(dz, lddz, N, SL_BF16), st));
     SHD_HIP(hipGetLastError());
+  } else if (short_dx) {
+    GemmArgs a = {};
+    a.A = dz; a.lda = lddz; a.B = d_w; a.ldb = ldw; a.M = M; a.N = K; a.K = N; a.C = d_dx; a.ldc = lddx;
+    SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
+    SHD_DISPATCH_16(dtype, short_launch<T>(a, st));
+    SHD_HIP(hipGetLastError());
   } else if (d_dx && M) {
     GemmArgs a = {};
     a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldp; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
-    a.K = act ? (uint32_t)ldp : N;           // (dz of an activation has zero pad columns, as W^T has: whole words)
+    a.K = need_dz ? (uint32_t)ldp : N;       // (pad columns are zero on both sides: whole words)
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
     SHD_DISPATCH_16(dtype, hipLaunchKernelGGL((transpose_kernel<T>), dim3((K + 31) / 32 * (uint32_t)((ldp + 31) / 32)), dim3(256), 0, st, (const T *)d_w, ldw, N, K,
                                               (T *)(ws + p.wt), ldp);
@@ -1419,10 +1552,9 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
     a.part = p.slices > 1 || narrow_dw ? reinterpret_cast<float *>(ws + p.part) : nullptr;
     a.part_b = d_db ? reinterpret_cast<float *>(ws + p.part_b) : nullptr;
     n.kept = static_cast<const char *>(d_kept); n.kept_act = act;
-    const bool da = act || dy_words;
     const uint64_t joined = (a.part ? (uint64_t)N * K : 0) + (d_db ? N : 0);
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dw_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, da, x_words, st);
+    SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, dz_words, x_words, st);
                     else if (bits_dw) tn_narrow_launch<T, true>(n, st);
                     else tn_narrow_launch<T, false>(n, st);
                     if (joined) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)((joined + 63) / 64)), dim3(256), 0, st, a.part, a.part_b, p.slices, N, K,

@@ -105,7 +105,7 @@ P = (C.addressof(_BUF) + 255) // 256 * 256          # a host address: the calls 
     ("sl_dropout", (1, P, 1 << 32, None, 0, 1, (1 << 31) + 8, 0.5, 1, None, P, 1 << 32, None)),        # columns are counted in 32 bits
     ("sl_linear16_fwd", (1, P, 4, P, 4, None, 0, None, 0, (1 << 31) - 1, 1, 4, 0, P, 1, None, None)),   # a launch of 2^32 threads and more
     ("sl_linear16_fwd", (1, P, 8, P, 8, None, 0, None, 0, (1 << 31) - 1, 1 << 24, 8, 0, P, 1 << 24, None, None)),
-    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 2, None, (1 << 31) - 1, 2, 8, 0, P, 8, None, 0, None, 0, P, None)),
+    ("sl_linear16_bwd", (1, P, 8, P, 8, P, 1 << 22, None, (1 << 31) - 1, 72, 8, 0, P, 8, None, 0, None, 0, P, None)),
     ("sl_linear16_bwd", (1, P, 1 << 24, P, 1 << 24, P, 1 << 24, None, 1, 1 << 24, 1 << 24, 0, P, 1 << 24, None, 0, None, 0, P, None)),
     ("sl_label_logprobs_fwd", (1, P, 2000, P, 1, 1 << 25, 2000, 0, P, P, P, None, None, None, None)),
 ])
