@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(256) lp_rows_kernel(LpArgs a) {
   if (sub == 0) answer_row(a, row, x, st, H);
   if (a.k == 0) return;
   // k rounds: the best remaining key of the group, then the lowest index that has it
+  const uint32_t rows = (uint32_t)__popcll(__ballot(true)) / L;         // of this wavefront
   int32_t key[NC][V];
 #pragma unroll
   for (int i = 0; i < NC; i++)
@@ -148,17 +149,31 @@ __global__ void __launch_bounds__(256) lp_rows_kernel(LpArgs a) {
 #pragma unroll
       for (int j = 0; j < V; j++) best = max(best, key[i][j]);
     best = (int32_t)group_all<L>((uint32_t)best, [](uint32_t p, uint32_t q) { return (uint32_t)max((int32_t)p, (int32_t)q); });
-    uint32_t at = 0xFFFFFFFFu;
+    uint32_t at = 0xFFFFFFFFu, hits = 0;                     // this lane's lowest index that has it; hits of the wavefront
+    bool hit[NC][V];
 #pragma unroll
     for (int i = NC - 1; i >= 0; i--)
 #pragma unroll
-      for (int j = V - 1; j >= 0; j--) at = key[i][j] == best ? (sub + i * L) * V + j : at;
-    at = group_all<L>(at, [](uint32_t p, uint32_t q) { return min(p, q); });
+      for (int j = V - 1; j >= 0; j--) {
+        hit[i][j] = key[i][j] == best;
+        hits += (uint32_t)__popcll(__ballot(hit[i][j]));
+        at = hit[i][j] ? (sub + i * L) * V + j : at;
+      }
+    bool mine = at != 0xFFFFFFFFu;
+    if (hits == rows) {                                      // (uniform) no ties: the compares above tell what to take out, its lane answers
 #pragma unroll
-    for (int i = 0; i < NC; i++)
+      for (int i = 0; i < NC; i++)
 #pragma unroll
-      for (int j = 0; j < V; j++) key[i][j] = (sub + i * L) * V + j == at ? kNoKey : key[i][j];
-    if (sub == r % L) {
+        for (int j = 0; j < V; j++) key[i][j] = hit[i][j] ? kNoKey : key[i][j];
+    } else {
+      const uint32_t first = group_all<L>(at, [](uint32_t p, uint32_t q) { return min(p, q); });
+      mine = at == first;
+#pragma unroll
+      for (int i = 0; i < NC; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) key[i][j] = (sub + i * L) * V + j == first ? kNoKey : key[i][j];
+    }
+    if (mine) {
       a.top_lp[row * a.k + r] = logprob_of(value_of(best), st);
       a.top_idx[row * a.k + r] = at;
     }
