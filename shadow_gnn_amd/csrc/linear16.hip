@@ -9,6 +9,9 @@
 // Tiles are staged in LDS 64 steps of the contraction at a time -- 128 bytes of every row: with half lines (32 steps) every line
 // crossed to the CU twice, 338 instead of 314 us at 32768 x 1024 x 4096 -- and multiplied on 32x32x16 products formed as W x^T: a lane then
 // holds four neighbouring output COLUMNS of a row.
+// 32768 x 1024 x 4096 fp16 gelu: 360 us, 215 of them the main loop (1.28 PFLOP/s; the products alone 166) and some 95 the epilogue, whose
+// gelu does not overlap with it.  289127 x 256 x 256 bf16 relu with residual (bound by memory): forward 105 us, dx 95, dW 83 + 12.
+// 256 x 256 x 256: 4.8 us.
 // Operands whose rows are whole 16-byte words go to LDS directly (global_load_lds, no registers); any other pitch or width is loaded
 // into registers (unaligned 16-byte loads, the last word of a row element by element) and written from there.
 #include "elem.h"

@@ -1,6 +1,7 @@
 // ops_mlp.cpp -- the host side of the node-wise MLP operators (shadow_gnn_amd/ops_mlp.py): argument checks, autograd nodes and the
 // calls of the C entries (include/shadow_hip.h).  Small calls are bound by the host, and a backward pass written in Python also waits
-// for the interpreter lock in autograd's thread: forward + backward of a layer norm of 64 x 64 takes 40 us here, 70 to 110 us so.
+// for the interpreter lock in autograd's thread: forward + backward of a layer norm of 64 x 64 takes 33 to 68 us here, 70 to 134 us so
+// (the spread is autograd's thread being woken).
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
