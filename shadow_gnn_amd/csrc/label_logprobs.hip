@@ -15,8 +15,8 @@
 // Two forms of the forward pass (forward_in_registers() has the rule): rows of up to 1024 classes stay in the registers of 4 to 64
 // lanes; longer ones are streamed by a workgroup each -- by several, joined by a second kernel, where there are few rows.
 // 289127 x 172 fp32: forward 32 us without alternatives (6.2 TB/s), 68 with five (each is a round of compares over the row's registers);
-// backward 70 us (5.7 TB/s).  2048 x 131072 bf16: forward 137 us (3.9 TB/s: eleven operations per element run beside the loads),
-// backward 177 us (6.1 TB/s).  1 x 131072 fp16 with ten alternatives: 8.4 + 7.0 us, the latency of two launches and of the lists.
+// backward 70 us (5.7 TB/s).  2048 x 131072 bf16: forward 99 us (5.4 TB/s; eleven operations per element run beside the
+// loads), backward 177 us (6.1 TB/s).  1 x 131072 fp16 with ten alternatives: 8.4 + 7.0 us, the latency of two launches and of the lists.
 #include "elem.h"
 
 using namespace shadow;
@@ -342,11 +342,13 @@ __device__ __forceinline__ void feed_top(const float (&v)[W][V], uint32_t base, 
 
 constexpr int kStreamThreads = 256, kStreamWords = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
+// TOP: with alternatives.  Without them the next trip's words are on their way while a trip is summed (2048 x 131072 bf16: 99 us, 117
+// through the form with lists, whose registers have no room for it).
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kStreamThreads, 4) lp_stream_kernel(LpArgs a) {
   constexpr int V = kVec<T>, W = kStreamWords, NW = kStreamThreads / 64;
   __shared__ float st[NW][3];
-  __shared__ int2 lists[NW * kMaxTop], places[NW][64];
+  __shared__ int2 lists[TOP ? NW * kMaxTop : 1], places[TOP ? NW : 1][64];
   const uint64_t row = blockIdx.x / a.splits;
   const uint32_t split = blockIdx.x % a.splits;
   const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.ldx;
@@ -358,48 +360,76 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
   float M = -INFINITY, S = 0.f, Tt = 0.f;
   Best b;
   best_init(b);
-  for (uint32_t w = w0; w < w1; w += kStreamThreads * W) {      // (uniform trips: the wavefront's list needs every lane)
-    float v[W][V];
+  if constexpr (!TOP) {
+    const Vec<T, V> *src = reinterpret_cast<const Vec<T, V> *>(x + head);
+    Vec<T, V> ahead[W];
+    auto fetch = [&](uint32_t w) {            // (past w1 the last word again: it is not used)
 #pragma unroll
-    for (int i = 0; i < W; i++) {
-      const uint32_t c = w + i * kStreamThreads + threadIdx.x;
+      for (int i = 0; i < W; i++) ahead[i] = src[min(w + i * kStreamThreads + threadIdx.x, w1 - 1)];
+    };
+    if (w0 < w1) fetch(w0);
+    for (uint32_t w = w0; w < w1; w += kStreamThreads * W) {
+      float v[W][V];
 #pragma unroll
-      for (int j = 0; j < V; j++) v[i][j] = -INFINITY;
-      if (c < w1) ldv<T, V>(x + head + (uint64_t)c * V, v[i]);
-    }
-    feed_stats<W, V>(v, M, S, Tt);
-    // (words past w1 are padding here: their index is put past C)
-    if (a.k) {
-      if (w == w0) {                                            // (uniform) the first trip
-        float best = -INFINITY;
+      for (int i = 0; i < W; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) v[i][j] = (float)ahead[i].v[j];
+      if (w + kStreamThreads * W < w1) {
+        fetch(w + kStreamThreads * W);
+      } else {
 #pragma unroll
         for (int i = 0; i < W; i++)
+          if (w + i * kStreamThreads + threadIdx.x >= w1) {
 #pragma unroll
-          for (int j = 0; j < V; j++) best = nan_max(best, v[i][j]);
-        b.floor = kth_of_lanes(w + threadIdx.x < w1 ? key_of(best) : kNoKey, a.k);
-        best_quick(b);
-        Collect col = {places[wave_id()], 0};
-#pragma unroll
-        for (int i = 0; i < W; i++) {
-          const uint32_t c = w + i * kStreamThreads + threadIdx.x;
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            const int32_t key = key_of(v[i][j]);
-            collect(col, c < w1 && key >= b.floor, key, (int32_t)(head + c * V + j));
+            for (int j = 0; j < V; j++) v[i][j] = -INFINITY;
           }
-        }
-        if (col.total <= 64) {
-          rank_collected(col, b, a.k);
-          continue;
-        }
       }
+      feed_stats<W, V>(v, M, S, Tt);
+    }
+  } else {
+    for (uint32_t w = w0; w < w1; w += kStreamThreads * W) {      // (uniform trips: the wavefront's list needs every lane)
+      float v[W][V];
 #pragma unroll
       for (int i = 0; i < W; i++) {
         const uint32_t c = w + i * kStreamThreads + threadIdx.x;
-        float one[1][V];
 #pragma unroll
-        for (int j = 0; j < V; j++) one[0][j] = v[i][j];
-        feed_top<1, V>(one, c < w1 ? head + c * V : a.C, 0, a.C, b, a.k);
+        for (int j = 0; j < V; j++) v[i][j] = -INFINITY;
+        if (c < w1) ldv<T, V>(x + head + (uint64_t)c * V, v[i]);
+      }
+      feed_stats<W, V>(v, M, S, Tt);
+      // (words past w1 are padding here: their index is put past C)
+      {
+        if (w == w0) {                                            // (uniform) the first trip
+          float best = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < W; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) best = nan_max(best, v[i][j]);
+          b.floor = kth_of_lanes(w + threadIdx.x < w1 ? key_of(best) : kNoKey, a.k);
+          best_quick(b);
+          Collect col = {places[wave_id()], 0};
+#pragma unroll
+          for (int i = 0; i < W; i++) {
+            const uint32_t c = w + i * kStreamThreads + threadIdx.x;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+              const int32_t key = key_of(v[i][j]);
+              collect(col, c < w1 && key >= b.floor, key, (int32_t)(head + c * V + j));
+            }
+          }
+          if (col.total <= 64) {
+            rank_collected(col, b, a.k);
+            continue;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const uint32_t c = w + i * kStreamThreads + threadIdx.x;
+          float one[1][V];
+#pragma unroll
+          for (int j = 0; j < V; j++) one[0][j] = v[i][j];
+          feed_top<1, V>(one, c < w1 ? head + c * V : a.C, 0, a.C, b, a.k);
+        }
       }
     }
   }
@@ -407,14 +437,15 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
     const uint32_t t = threadIdx.x, c = t < head ? t : tail0 + (t - head);
     float one[1][1] = {{c < a.C && t < 2 * V ? (float)x[c < a.C ? c : 0] : -INFINITY}};
     feed_stats<1, 1>(one, M, S, Tt);
-    if (a.k) feed_top<1, 1>(one, t < 2 * V ? c : a.C, 0, a.C, b, a.k);
+    if (TOP) feed_top<1, 1>(one, t < 2 * V ? c : a.C, 0, a.C, b, a.k);
   }
   // lanes -> wavefront -> workgroup
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1)
     join_stats(M, S, Tt, __shfl_xor(M, off, 64), __shfl_xor(S, off, 64), __shfl_xor(Tt, off, 64));
   if (lane_id() == 0) { st[wave_id()][0] = M; st[wave_id()][1] = S; st[wave_id()][2] = Tt; }
-  if (a.splits > 1) {                         // (the wavefronts' lists go to the join as they are)
+  if (!TOP) {
+  } else if (a.splits > 1) {                  // (the wavefronts' lists go to the join as they are)
     if (lane_id() < a.k) a.part_top[((row * a.splits + split) * NW + wave_id()) * a.k + lane_id()] = make_int2(b.key, b.idx);
   } else if (lane_id() < a.k) {
     lists[wave_id() * a.k + lane_id()] = make_int2(b.key, b.idx);
@@ -429,11 +460,11 @@ __global__ void __launch_bounds__(kStreamThreads) lp_stream_kernel(LpArgs a) {
     }
     return;
   }
-  if (a.k) b = best_of(NW * a.k, a.k, places[0], [&](uint32_t e) { return lists[e]; });
+  if (TOP) b = best_of(NW * a.k, a.k, places[0], [&](uint32_t e) { return lists[e]; });
   float H;
   const float2 stat = finish_stats(M, S, Tt, H);
   if (lane_id() == 0) answer_row(a, row, x, stat, H);
-  if (lane_id() < a.k) {
+  if (TOP && lane_id() < a.k) {
     a.top_lp[row * a.k + lane_id()] = logprob_of(value_of(b.key), stat);
     a.top_idx[row * a.k + lane_id()] = b.idx;
   }
@@ -580,7 +611,8 @@ void rows_dispatch(const LpArgs &a, hipStream_t st) {
 
 template <typename T>
 void stream_launch(const LpArgs &a, hipStream_t st) {
-  hipLaunchKernelGGL((lp_stream_kernel<T>), dim3(a.n * a.splits), dim3(kStreamThreads), 0, st, a);
+  if (a.k) hipLaunchKernelGGL((lp_stream_kernel<T, true>), dim3(a.n * a.splits), dim3(kStreamThreads), 0, st, a);
+  else hipLaunchKernelGGL((lp_stream_kernel<T, false>), dim3(a.n * a.splits), dim3(kStreamThreads), 0, st, a);
   if (a.splits > 1) hipLaunchKernelGGL((lp_join_kernel<T>), dim3(a.n), dim3(kStreamThreads), 0, st, a);
 }
 

@@ -42,6 +42,15 @@ __device__ __forceinline__ void normal_cdf(float z, float &cdf, float &ex) {
   const float q = 0.5f * ex * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
   cdf = z > 0.f ? 1.f - q : q;
 }
+// z Phi(z) = max(z, 0) - |z| q, q the tail beyond |z|.  (|z| held below 64, where the tail has long been zero: no 0 * inf; a NaN comes
+// through the maximum.)
+__device__ __forceinline__ float gelu(float z) {
+  const float az = fminf(fabsf(z), 64.f);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(az, 0.3275911f * 0.70710678f, 1.f));
+  const float w = az * 0.84932180f;          // (w^2 = z^2 / 2 log2 e)
+  const float q = __builtin_amdgcn_exp2f(-w * w) * t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  return __builtin_fmaf(-az, q, __builtin_elementwise_maximum(z, 0.f));
+}
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
 __device__ __forceinline__ float tanh16(float z) {            // exp2 form; near zero, where it cancels, two series terms
   const float s = z * (1.f - z * z * 0.33333333f);
@@ -51,7 +60,7 @@ __device__ __forceinline__ float tanh16(float z) {            // exp2 form; near
 __device__ __forceinline__ float act16(int act, float z) {
   switch (act) {
     case 3: return tanh16(z);
-    case kActGelu: { float c, e; normal_cdf(z, c, e); return z == -INFINITY ? 0.f : z * c; }
+    case kActGelu: return gelu(z);
     case kActSilu: return z == -INFINITY ? 0.f : z * sigmoid(z);
     default: return act_fwd(act, z);
   }
