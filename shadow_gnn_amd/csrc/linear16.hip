@@ -9,8 +9,8 @@
 // Tiles are staged in LDS 64 steps of the contraction at a time -- 128 bytes of every row: with half lines (32 steps) every line
 // crossed to the CU twice, 338 instead of 314 us at 32768 x 1024 x 4096 -- and multiplied on 32x32x16 products formed as W x^T: a lane then
 // holds four neighbouring output COLUMNS of a row.
-// 32768 x 1024 x 4096 fp16 gelu: 360 us, 215 of them the main loop (1.28 PFLOP/s; the products alone 166) and some 95 the epilogue, whose
-// gelu does not overlap with it.  289127 x 256 x 256 bf16 relu with residual (bound by memory): forward 105 us, dx 95, dW 83 + 12.
+// 32768 x 1024 x 4096 fp16 gelu: 352 us, 215 to 226 of them the main loop (1.2 PFLOP/s; the products alone 166, and LDS is busy as long)
+// and the rest an epilogue that does not overlap with it (two workgroups per CU of 128 x 256 tiles and half stages, whose would: 412).  289127 x 256 x 256 bf16 relu with residual (bound by memory): forward 105 us, dx 95, dW 83 + 12.
 // 256 x 256 x 256: 4.8 us.
 // Operands whose rows are whole 16-byte words go to LDS directly (global_load_lds, no registers); any other pitch or width is loaded
 // into registers (unaligned 16-byte loads, the last word of a row element by element) and written from there.
@@ -1388,14 +1388,16 @@ void short_launch(const GemmArgs &a, hipStream_t st) {
   hipLaunchKernelGGL((nt_short_kernel<T>), dim3((uint32_t)((items + 3) / 4)), dim3(256), 0, st, a, groups, per);
 }
 
+// the grid of 32 x 32 tiles: a launch has fewer than 2^32 threads
+bool few_fits(uint32_t M, uint32_t N) { return (((uint64_t)M + 31) / 32) * (((uint64_t)N + 31) / 32) < 1u << 23; }
 // x W^T in 32 x 32 tiles: fewer than 64 tiles of 128 (1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128
-// ones, twice the rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47); and what the tile kernel does not
+// ones, twice the rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47), fewer than 128 where half of each were
+// empty (8192 x 1024 -> 40 9.1 and 17.6, 16000 x 500 -> 48 9.4 and 12.8, but 16000 x 2000 -> 64 37 and 32), any number where three quarters
+// were (30000 x 500 -> 16 8.9 and 14.8, 100000 x 600 -> 8 27 and 38, but 60000 x 1000 -> 32 39 and 31); and what the tile kernel does not
 // hold: its offsets (256 rows of a pitch below 2^22 elements stay below 2^31 bytes) and contractions of less than eight, both rare
 bool takes_few(uint32_t M, uint32_t N, uint32_t K, int64_t lda, int64_t ldb) {
-  return tiles128(M, N) < 64 || lda >= (1 << 22) || ldb >= (1 << 22) || K < 8;
+  return tiles128(M, N) < (N <= 64 && K <= 1024 ? 128u : 64u) || (N <= 32 && K <= 640 && few_fits(M, N)) || lda >= (1 << 22) || ldb >= (1 << 22) || K < 8;
 }
-// its grid: a launch has fewer than 2^32 threads
-bool few_fits(uint32_t M, uint32_t N) { return (((uint64_t)M + 31) / 32) * (((uint64_t)N + 31) / 32) < 1u << 23; }
 
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
