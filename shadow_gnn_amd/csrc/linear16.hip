@@ -1290,9 +1290,12 @@ __global__ void __launch_bounds__(256) transpose_kernel(const T *W, int64_t ldw,
     if (k0 + r + i < K && n0 + c < ld) out[(int64_t)(k0 + r + i) * ld + n0 + c] = tile[c][r + i];
 }
 
-// the tall, narrow form: widths up to 256, the contraction's in whole words (a gradient's dz is: pad columns), rows for two 32-row
-// tiles per CU
-bool narrow_shape(uint32_t M, uint32_t N, uint32_t K) { return N <= 256 && K <= 256 && K % 8 == 0 && M >= 16384; }
+// the tall, narrow form: widths up to 256, the contraction's in whole words (a gradient's dz is: pad columns).  8192 x 256 -> 256 takes 8.4
+// us (dx 9.4) so and 10.2 (12.7) in 128 x 128 tiles, 32768 rows 15 (16) and 14 (17), 289127 105 and 140; fewer rows leave CUs idle.
+bool narrow_shape(uint32_t M, uint32_t N, uint32_t K) { return N <= 256 && K <= 256 && K % 8 == 0 && M >= 8192; }
+// ... of dz^T x, where 128 x 128 tiles would read an operand twice: dx and dW of 131072 x 256 -> 256 relu take 91 us so and 101 in tiles,
+// 65536 rows 64 and 58, 131072 x 64 -> 64 (one tile) 55 and 37
+bool narrow_dw_shape(uint32_t M, uint32_t N, uint32_t K) { return narrow_shape(M, N, K) && M >= 98304 && (N > 128 || K > 128); }
 // dx of so few outputs goes through nt_short_kernel (its wavefronts hold 64 steps of the contraction)
 constexpr uint32_t kShort = 64;
 
@@ -1359,8 +1362,7 @@ template <typename T, bool BITS>
 void tn_narrow_launch(const TnNarrowArgs &n, hipStream_t st) {
   const dim3 g(n.t.slices);
   if (n.t.N <= 128) {
-    if (n.t.K <= 128) hipLaunchKernelGGL((tn_narrow_kernel<T, 1, 2, 4, BITS>), g, dim3(128), 0, st, n);
-    else hipLaunchKernelGGL((tn_narrow_kernel<T, 1, 4, 4, BITS>), g, dim3(256), 0, st, n);
+    hipLaunchKernelGGL((tn_narrow_kernel<T, 1, 4, 4, BITS>), g, dim3(256), 0, st, n);      // (K > 128)
   } else {
     if (n.t.K <= 128) hipLaunchKernelGGL((tn_narrow_kernel<T, 2, 2, 4, BITS>), g, dim3(256), 0, st, n);
     else hipLaunchKernelGGL((tn_narrow_kernel<T, 2, 4, 4, BITS>), g, dim3(512), 0, st, n);
@@ -1476,7 +1478,7 @@ extern "C" size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N) {
 
 extern "C" size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K) {
   (void)act;
-  const uint64_t a = plan_bwd(M, N, K, false).total, b = narrow_shape(M, N, K) ? plan_bwd(M, N, K, true).total : 0;
+  const uint64_t a = plan_bwd(M, N, K, false).total, b = narrow_dw_shape(M, N, K) ? plan_bwd(M, N, K, true).total : 0;
   return a > b ? a : b;
 }
 
@@ -1496,7 +1498,7 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
   // a dy of few columns whose rows are not whole words is first laid out in such rows: loads of unaligned rows, many times over, cost
   // more (dx and dW of 20011 x 47 -> 500: 43 us so, 35 with the pass; 289127 x 47 -> 256: 152 and 117; 289127 x 172 -> 128: 120 and 133)
   const bool pad = !act && !dy_words && N <= kShort, dz_words = act || pad || dy_words;
-  const bool narrow_dx = d_dx && shape && dz_words, narrow_dw = want_w && shape && x_words && dz_words;
+  const bool narrow_dx = d_dx && shape && dz_words, narrow_dw = want_w && narrow_dw_shape(M, N, K) && x_words && dz_words;
   const bool bits_dw = narrow_dw && keeps_bits(act) && dy_words;       // (dz^T x masks dy itself)
   const bool few_dx = d_dx && M && !narrow_dx && tiles128(M, K) < 64, few_dw = want_w && M && !narrow_dw && few_rows(M, N, K),
              short_dx = d_dx && M && !narrow_dx && !few_dx && N <= kShort && ldw < (1 << 22);

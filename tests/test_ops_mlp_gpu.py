@@ -325,6 +325,17 @@ def test_linear_act_tall_and_narrow(dtype, act, M, N, K):
     _lin_check(x, W, _randn(g, N), act, _randn(g, M, N, dtype=dtype), _randn(g, M, N, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["I", "relu", "leakyrelu", "silu"])
+@pytest.mark.parametrize("M,N,K", [(98304, 256, 256), (98311, 136, 128), (98335, 96, 200), (100003, 250, 144), (98321, 47, 160)])
+def test_linear_act_all_of_the_weight_gradient_at_once(dtype, act, M, N, K):
+    """Rows enough for one workgroup to hold all of dW; operands pitched, and dy in rows of whole words and not."""
+    g = _gen(M + N + K)
+    x, W, dy = _randn(g, M, K, dtype=dtype), _randn(g, N, K, dtype=dtype, scale=K ** -0.5), _randn(g, M, N, dtype=dtype)
+    _lin_check(_pitched(x, K + 8), W, _randn(g, N), act, None, _pitched(dy, N // 8 * 8 + 16))
+    _lin_check(x, W, None, act, None, dy)
+
+
 @pytest.mark.parametrize("act", ["I", "relu", "tanh"])
 def test_linear_act_tall_and_narrow_in_parts(act):
     """Single gradients, pitched operands and rows that are no whole words: the forms mix."""
@@ -626,6 +637,7 @@ def test_rows_behind_the_last_stay_as_they_were():
 
 
 @pytest.mark.parametrize("M,N,K,act", [
+    (98309, 256, 256, 1), (98309, 136, 72, 5), (98309, 72, 136, 0), (98309, 47, 256, 0),       # dz^T x of all of dW at once
     (16411, 256, 256, 1), (16411, 128, 72, 5), (16387, 72, 136, 4), (16393, 40, 16, 0),      # tall, narrow: whole words
     (1111, 1100, 264, 2), (1111, 1100, 263, 1),                                             # 128 x 128 tiles, words and any rows
     (4100, 4200, 520, 6),                                                                   # 256 x 256 tiles
