@@ -110,16 +110,17 @@ Tensor like(const Tensor &x, at::IntArrayRef shape) { return at::empty(shape, x.
 Tensor like(const Tensor &x, at::IntArrayRef shape, at::ScalarType t) { return at::empty(shape, x.options().dtype(t).requires_grad(false)); }
 
 // A gradient of these operators is not differentiable itself: with create_graph its own backward pass is an error, not a silent zero.
+// Its inputs are x and dy, and what a gradient depends on where both of them are constants (w, b: they stand in act'(z)).
 struct Once : public Function<Once> {
-  static Tensor forward(AutogradContext *, const Tensor &g, const Tensor &, const Tensor &) { return g.view_as(g); }
+  static Tensor forward(AutogradContext *, const Tensor &g, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &) { return g.view_as(g); }
   static variable_list backward(AutogradContext *, const variable_list &) {
     TORCH_CHECK(false, "the operators of shadow_gnn_amd.ops_mlp are differentiable once");
   }
 };
-void once(variable_list &grads, const Tensor &x, const Tensor &dy) {
+void once(variable_list &grads, const Tensor &x, const Tensor &dy, const OptTensor &w = {}, const OptTensor &b = {}) {
   if (!at::GradMode::is_enabled()) return;
   for (Tensor &g : grads)
-    if (g.defined()) g = Once::apply(g, x, dy);
+    if (g.defined()) g = Once::apply(g, x, dy, w, b);
 }
 
 // ------------------------------------------------------------------------------------------------ layer norm
@@ -258,6 +259,8 @@ struct LinearAct : public Function<LinearAct> {
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b ? (int64_t)b->scalar_type() : (int64_t)-1;
     ctx->saved_data["residual"] = residual.has_value();
+    // (for once() alone, which reads no value of it: not a saved tensor, which must not change before the backward pass)
+    if (act && needs_grad(b)) ctx->saved_data["b"] = *b;
     ctx->save_for_backward({x, W, kept});
     return y;
   }
@@ -284,7 +287,8 @@ struct LinearAct : public Function<LinearAct> {
                             bias == (int64_t)at::kFloat, ws.data_ptr(), on.stream));
       if (need_w) out[1] = dW;
     }
-    once(out, x, dy);
+    const auto b = ctx->saved_data.find("b");
+    once(out, x, dy, act ? OptTensor(W) : OptTensor(), b != ctx->saved_data.end() ? OptTensor(b->second.toTensor()) : OptTensor());
     if (need_r) out[3] = dy;
     return out;
   }

@@ -684,6 +684,38 @@ def test_gradients_are_differentiable_once():
         first.float().sum().backward()
 
 
+@pytest.mark.parametrize("act", ["relu", "elu", "tanh", "leakyrelu", "gelu", "silu"])
+@pytest.mark.parametrize("which", ["weight", "bias"])
+def test_gradients_of_a_first_layer_are_differentiable_once(act, which):
+    """Raw features and a constant dy: dW and db still depend on the weight and the bias, through act'(z)."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(61)
+    x, W, b = _randn(g, 64, 48, dtype=BF16), _randn(g, 40, 48, dtype=BF16, scale=0.1), _randn(g, 40)
+    leaf = (W if which == "weight" else b).requires_grad_(True)
+    y = ops_mlp.linear_act(x, W, b, act=act)
+    plain, = torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+    first, = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+    assert torch.equal(first.detach(), plain)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (y.float().sum() + first.float().square().sum()).backward()
+    # an identity's gradients of constants are constants: the penalty adds nothing, here as in torch
+    y = ops_mlp.linear_act(x, W, b)
+    first, = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+    got, = torch.autograd.grad(y.float().sum() + first.float().square().sum(), leaf)
+    assert torch.equal(got, first)
+
+
+def test_a_bias_may_change_before_the_backward_pass():
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(62)
+    x, W, b, dy = _randn(g, 64, 48, dtype=BF16), _randn(g, 40, 48, dtype=BF16, scale=0.1), _randn(g, 40).requires_grad_(True), _randn(g, 64, 40, dtype=BF16)
+    want, = torch.autograd.grad(ops_mlp.linear_act(x, W, b, act="gelu"), b, dy)
+    y = ops_mlp.linear_act(x, W, b, act="gelu")
+    with torch.no_grad():
+        b.add_(1)
+    assert torch.equal(torch.autograd.grad(y, b, dy)[0], want)
+
+
 def test_one_tensor_in_several_places():
     """Scale and offset, x and residual, x and weight may be one tensor: its gradient is the sum of both places'."""
     from shadow_gnn_amd import ops_mlp
