@@ -64,6 +64,14 @@ void one_device(const Tensor &t, const OptTensor &o, const More &...more) {
   one_device(t, more...);
 }
 
+// Forward-mode derivatives are not provided: a tangent, of an input or of a gradient, is an error, not a silent zero.
+void no_tangents(const char *) {}
+template <typename... More>
+void no_tangents(const char *name, const OptTensor &t, const More &...more) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), name, ": forward-mode derivatives are not provided");
+  no_tangents(name, more...);
+}
+
 bool needs_grad(const Tensor &t) { return t.requires_grad(); }
 bool needs_grad(const OptTensor &t) { return t && t->requires_grad(); }
 template <typename... Ts>
@@ -148,6 +156,7 @@ struct LayerNorm : public Function<LayerNorm> {
   static variable_list backward(AutogradContext *ctx, const variable_list &dys) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &scale = saved[1], &offset = saved[2], &stats = saved[3], &dy = dys[0];
+    no_tangents("layer_norm", dy);
     size_t edge = 0;
     const bool need_x = ctx->needs_input_grad(edge++), need_s = scale.defined() && ctx->needs_input_grad(edge++), need_o = offset.defined() && ctx->needs_input_grad(edge++);
     variable_list out(4);
@@ -182,6 +191,7 @@ Tensor layer_norm(const Tensor &x, const OptTensor &scale, const OptTensor &offs
       if ((*t)->dim() != 1 || (*t)->size(0) != F) value_error("layer_norm: scale / offset " + say(**t) + " for rows of " + std::to_string(F));
     }
   if (scale && offset && scale->scalar_type() != offset->scalar_type()) type_error("layer_norm: scale " + say(*scale) + " and offset " + say(*offset));
+  no_tangents("layer_norm", x, scale, offset);
   one_device(x, scale, offset);
   const OptTensor s = scale ? OptTensor(scale->contiguous()) : scale, o = offset ? OptTensor(offset->contiguous()) : offset;
   if (any_grad(x, s, o)) return LayerNorm::apply(x, s, o, eps);
@@ -209,6 +219,7 @@ struct Dropout : public Function<Dropout> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &dys) {
     const Tensor d_seed = ctx->get_saved_variables()[0], &dy = dys[0];
+    no_tangents("dropout", dy);
     const bool residual = ctx->saved_data["residual"].toBool();
     variable_list out(5);
     if (ctx->needs_input_grad(0)) {
@@ -227,6 +238,7 @@ Tensor dropout(const Tensor &x, double p, uint64_t seed, const OptTensor &d_seed
   if (!((float)p < 1.0f)) value_error("dropout: the probability rounds to 1 in fp32");
   if (residual && (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type())) value_error("dropout: residual " + say(*residual) + " for x " + say(x));
   if (d_seed && (d_seed->scalar_type() != at::kLong || d_seed->numel() != 1)) value_error("dropout: a seed tensor is one int64");
+  no_tangents("dropout", x, residual);
   one_device(x, residual, d_seed);
   if (any_grad(x, residual)) return Dropout::apply(x, residual, d_seed, p, (int64_t)seed);
   return drop(x, p, seed, d_seed, residual);
@@ -267,6 +279,7 @@ struct LinearAct : public Function<LinearAct> {
   static variable_list backward(AutogradContext *ctx, const variable_list &dys) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &W = saved[1], &kept = saved[2], &dy = dys[0];
+    no_tangents("linear_act", dy);
     const int act = (int)ctx->saved_data["act"].toInt();
     const int64_t bias = ctx->saved_data["bias"].toInt();
     size_t edge = 2;
@@ -305,6 +318,7 @@ Tensor linear_act(const Tensor &x, const Tensor &W, const OptTensor &b, int64_t 
     value_error("linear_act: bias " + say(*b) + " for " + std::to_string(N) + " outputs of " + say(x));
   if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != at::IntArrayRef(out_shape(x, N))))
     value_error("linear_act: residual " + say(*residual) + " for " + std::to_string(N) + " outputs of x " + say(x));
+  no_tangents("linear_act", x, W, b, residual);
   one_device(x, OptTensor(W), b, residual);
   const OptTensor bc = b ? OptTensor(b->contiguous()) : b;
   if (any_grad(x, W, bc, residual)) return LinearAct::apply(x, W, bc, residual, act);
@@ -345,6 +359,7 @@ struct LabelLogprobs : public Function<LabelLogprobs> {
     if (!dys[0].defined() && !dys[1].defined() && !dys[2].defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &label = saved[1], &ent = saved[2], &idx = saved[3], &stat = saved[4];
+    no_tangents("label_logprobs", dys[0], dys[1], dys[2]);
     const uint32_t k = (uint32_t)ctx->saved_data["k"].toInt();
     {
       at::NoGradGuard no_grad;
@@ -371,6 +386,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> label_logprobs(const Tensor &x, const
   if ((label.scalar_type() != at::kInt && label.scalar_type() != at::kLong) || label.sizes() != x.sizes().slice(0, x.dim() - 1))
     value_error("label_logprobs: label " + say(label) + " for logits " + say(x));
   if (C < 1 || k < 0 || k > C || k > 64) value_error("label_logprobs: topk " + std::to_string(k) + " of " + std::to_string(C) + " classes (at most 64)");
+  no_tangents("label_logprobs", x);
   one_device(x, OptTensor(label));
   const Tensor lab = label.contiguous();
   const variable_list o = any_grad(x) ? LabelLogprobs::apply(x, lab, k) : lp_forward(x, lab, k);

@@ -4,8 +4,9 @@
 They stand beside the fp32 operators of ``ops`` (act_norm, the fused dropouts, linear, node_head): the pieces of a residual block
 ``x + dropout(linear_act(linear_act(layer_norm(x), W1, b1, "gelu"), W2, b2))`` over node embeddings, and of its answers.  Every
 operator takes ``[..., width]`` tensors on a ROCm device (rows of any pitch and alignment; other strides are copied), runs on the
-current stream of that device, keeps its sums and statistics in fp32, is differentiable once in every floating input, allocates through
-torch (so it may be captured into a graph) and gives the same bits on every call.  No CPU / torch fallback.
+current stream of that device, keeps its sums and statistics in fp32, is differentiable once in every floating input (a second backward
+pass raises RuntimeError, a forward-mode tangent NotImplementedError), allocates through torch (so it may be captured into a graph) and
+gives the same bits on every call.  No CPU / torch fallback.
 
 The checks, autograd nodes and calls of the C entries are in csrc/ops_mlp.cpp: small calls are bound by the host.
 """

@@ -4,6 +4,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from shadow_gnn_amd import _lib, ops_mlp
 
@@ -62,6 +63,27 @@ def _t(*shape, dtype=BF16):
 def test_python_entries_refuse(call, error):
     with pytest.raises(error):
         call()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call,shape", [
+    (lambda t: ops_mlp.layer_norm(t), (4, 8)),
+    (lambda t: ops_mlp.layer_norm(_t(4, 8, dtype=F32), t), (8,)),
+    (lambda t: ops_mlp.layer_norm(_t(4, 8, dtype=F32), _t(8, dtype=F32), t), (8,)),
+    (lambda t: ops_mlp.dropout(t, 0.5, 1), (4, 8)),
+    (lambda t: ops_mlp.dropout(_t(4, 8, dtype=F32), 0.5, 1, residual=t), (4, 8)),
+    (lambda t: ops_mlp.linear_act(t.to(BF16), _t(5, 8)), (4, 8)),
+    (lambda t: ops_mlp.linear_act(_t(4, 8), t.to(BF16)), (5, 8)),
+    (lambda t: ops_mlp.linear_act(_t(4, 8), _t(5, 8), t), (5,)),
+    (lambda t: ops_mlp.linear_act(_t(4, 8), _t(5, 8), residual=t.to(BF16)), (4, 5)),
+    (lambda t: ops_mlp.label_logprobs(t, torch.zeros(4, dtype=torch.int64)), (4, 8)),
+])
+def test_forward_mode_tangents_are_refused(call, shape, grad):
+    """A tangent of any floating input, also where nothing requires a gradient: an error, not an output without one."""
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = forward_ad.make_dual(torch.zeros(*shape), torch.ones(*shape))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
 
 
 _BUF = (C.c_char * 4096)()

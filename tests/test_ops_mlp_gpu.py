@@ -5,6 +5,7 @@ computation may lose, u = 2^-24 per operation on the magnitudes that enter it; e
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -714,6 +715,22 @@ def test_a_bias_may_change_before_the_backward_pass():
     with torch.no_grad():
         b.add_(1)
     assert torch.equal(torch.autograd.grad(y, b, dy)[0], want)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent of an input or of the gradient that a backward pass starts from: an error, not zeros."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(63)
+    x, W, s, label = _randn(g, 64, 64, dtype=BF16), _randn(g, 64, 64, dtype=BF16, scale=0.1), _randn(g, 64), torch.zeros(64, dtype=torch.int64, device=DEV)
+    for f in (lambda t: ops_mlp.layer_norm(t, s, s), lambda t: ops_mlp.dropout(t, 0.5, 3), lambda t: ops_mlp.linear_act(t, W, s, act="gelu"),
+              lambda t: ops_mlp.label_logprobs(t, label, topk=2).entropy):
+        for leaf in (x, x.clone().requires_grad_(True)):
+            with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f(forward_ad.make_dual(leaf, torch.ones_like(x)))
+        y = f(leaf)
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+        assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == x.shape
 
 
 def test_one_tensor_in_several_places():
