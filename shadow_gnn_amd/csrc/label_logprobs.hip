@@ -536,6 +536,7 @@ __device__ __forceinline__ RowGrad row_grad(const LpBwdArgs &a, uint64_t row) {
   if (a.dtop)
     for (uint32_t j = 0; j < a.k; j++) g.neg += a.dtop[row * a.k + j];
   g.dead = g.M == -INFINITY;
+  if (g.dead) g.a = g.h = g.neg = 0.f;                   // (a loss may hand such a row's -inf an infinite gradient: no 0 * inf)
   return g;
 }
 // the gradient of one element without its one-hot terms

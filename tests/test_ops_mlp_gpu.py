@@ -562,6 +562,24 @@ def test_label_logprobs_masks_ties_and_special_rows(dtype, C):
     assert not dy[0].any() and not dy[3].any() and dy[1].isfinite().all() and dy[2].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("C", [47, 172, 3000])
+def test_label_logprobs_rows_without_a_finite_logit_have_gradient_zero(dtype, C):
+    """... whatever comes back for their scores: a square of -inf has an infinite gradient, its mean over nothing a NaN."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(46)
+    x = _randn(g, 5, C, dtype=dtype)
+    x[1:4] = float("-inf")
+    x.requires_grad_(True)
+    out = ops_mlp.label_logprobs(x, torch.tensor([1, 2, -1, C - 1, 0], device=DEV), topk=2)
+    dx, = torch.autograd.grad(out.logprob.square().sum() + out.top_logprob.square().sum(), x, retain_graph=True)
+    assert not dx[1:4].any() and dx[[0, 4]].isfinite().all() and dx[[0, 4]].any(1).all()
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        a, h, t = torch.full((5,), bad, device=DEV), torch.full((5,), bad, device=DEV), torch.full((5, 2), bad, device=DEV)
+        dx, = torch.autograd.grad([out.logprob, out.entropy, out.top_logprob], x, [a, h, t], retain_graph=True)
+        assert not dx[1:4].any() and dx[[0, 4]].isnan().any(1).all()
+
+
 def test_label_logprobs_strides_and_shapes():
     from shadow_gnn_amd import ops_mlp
     g = _gen(44)
