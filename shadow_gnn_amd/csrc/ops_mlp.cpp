@@ -77,13 +77,17 @@ bool needs_grad(const OptTensor &t) { return t && t->requires_grad(); }
 template <typename... Ts>
 bool any_grad(const Ts &...ts) { return at::GradMode::is_enabled() && (needs_grad(ts) || ...); }
 
+// the tensor whose memory holds its values (the imaginary part of a conjugate is a view that negates)
+Tensor in_memory(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // [rows, width] with unit stride along the row and a pitch of at least the width (copied if it has neither)
 struct Rows {
   Tensor keep;
   void *p = nullptr;
   int64_t n = 0, F = 0, ld = 0;
 };
-Rows rows_of(const Tensor &t) {
+Rows rows_of(const Tensor &given) {
+  const Tensor t = in_memory(given);
   Rows r;
   r.F = t.size(-1);
   r.n = 1;
@@ -193,7 +197,7 @@ Tensor layer_norm(const Tensor &x, const OptTensor &scale, const OptTensor &offs
   if (scale && offset && scale->scalar_type() != offset->scalar_type()) type_error("layer_norm: scale " + say(*scale) + " and offset " + say(*offset));
   no_tangents("layer_norm", x, scale, offset);
   one_device(x, scale, offset);
-  const OptTensor s = scale ? OptTensor(scale->contiguous()) : scale, o = offset ? OptTensor(offset->contiguous()) : offset;
+  const OptTensor s = scale ? OptTensor(in_memory(*scale).contiguous()) : scale, o = offset ? OptTensor(in_memory(*offset).contiguous()) : offset;
   if (any_grad(x, s, o)) return LayerNorm::apply(x, s, o, eps);
   return ln_forward(x, s, o, eps, nullptr);
 }
@@ -320,7 +324,7 @@ Tensor linear_act(const Tensor &x, const Tensor &W, const OptTensor &b, int64_t 
     value_error("linear_act: residual " + say(*residual) + " for " + std::to_string(N) + " outputs of x " + say(x));
   no_tangents("linear_act", x, W, b, residual);
   one_device(x, OptTensor(W), b, residual);
-  const OptTensor bc = b ? OptTensor(b->contiguous()) : b;
+  const OptTensor bc = b ? OptTensor(in_memory(*b).contiguous()) : b;
   if (any_grad(x, W, bc, residual)) return LinearAct::apply(x, W, bc, residual, act);
   return lin_forward(x, W, bc, residual, (int)act, nullptr);
 }
@@ -365,7 +369,7 @@ struct LabelLogprobs : public Function<LabelLogprobs> {
       at::NoGradGuard no_grad;
       Tensor g[3];
       for (int i = 0; i < 3; i++)
-        if (dys[i].defined() && dys[i].numel()) g[i] = dys[i].contiguous();
+        if (dys[i].defined() && dys[i].numel()) g[i] = in_memory(dys[i]).contiguous();
       const Rows r = rows_of(x);
       out[0] = like(x, x.sizes());
       if (r.n) {

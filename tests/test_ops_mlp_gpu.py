@@ -820,6 +820,39 @@ def test_offsets_past_32_bits():
     assert torch.equal(y[-2:], torch.where(kept, base[:2, :F] * 2, torch.zeros((), dtype=BF16, device=DEV)))
 
 
+def test_negating_views():
+    """The imaginary part of a conjugate negates on reading; rows of one element and vectors of one are taken without a copy."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(64)
+
+    def view(*shape):
+        t = torch.complex(_randn(g, *shape), _randn(g, *shape)).conj().imag
+        assert t.is_neg()
+        return t
+
+    def same(f, *views):
+        def run(ts):
+            ts = [t.detach().requires_grad_(True) for t in ts]
+            y = f(*ts)
+            return (y,) + torch.autograd.grad(y, ts, y.detach())
+        for a, b in zip(run(views), run([t.resolve_neg() for t in views])):
+            assert torch.equal(a, b)
+
+    label = torch.zeros(9, dtype=torch.int64, device=DEV)
+    same(lambda x, s, o: ops_mlp.layer_norm(x, s, o), view(9, 1), view(1), view(1))
+    same(lambda x, r: ops_mlp.dropout(x, 0.25, 3, residual=r), view(9, 1), view(9, 1))
+    same(lambda b: ops_mlp.linear_act(torch.ones(9, 8, dtype=BF16, device=DEV), torch.ones(1, 8, dtype=BF16, device=DEV), b, act="gelu").float(), view(1))
+    same(lambda x: ops_mlp.label_logprobs(x, label).logprob, view(9, 1))
+    same(lambda x: ops_mlp.label_logprobs(x, label).entropy, view(9, 5))
+    x = _randn(g, 9, 1).requires_grad_(True)
+    dy = view(9, 1)
+    assert torch.equal(*[torch.autograd.grad(ops_mlp.dropout(x, 0.0, 1), x, t)[0] for t in (dy, dy.resolve_neg())])
+    x = _randn(g, 5).requires_grad_(True)
+    dy = view(5)[2]
+    out = ops_mlp.label_logprobs(x, torch.tensor(3, device=DEV)).logprob
+    assert torch.equal(*[torch.autograd.grad(out, x, t, retain_graph=True)[0] for t in (dy, dy.resolve_neg())])
+
+
 def test_other_streams():
     from shadow_gnn_amd import ops_mlp
     g = _gen(53)
