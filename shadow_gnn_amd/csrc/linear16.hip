@@ -65,15 +65,13 @@ __device__ __forceinline__ float act16(int act, float z) {
     default: return act_fwd(act, z);
   }
 }
+// act'(z) of the activations that keep z (relu and leakyrelu keep a bit of it)
 __device__ __forceinline__ float slope16(int act, float z) {
   switch (act) {
-    case 1: return z > 0.f ? 1.f : 0.f;
     case 2: return z > 0.f ? 1.f : __builtin_amdgcn_exp2f(z * 1.44269504f);
     case 3: { const float h = tanh16(z); return 1.f - h * h; }
-    case 4: return z > 0.f ? 1.f : 0.2f;
     case kActGelu: { float c, e; normal_cdf(z, c, e); return fabsf(z) == INFINITY ? c : c + z * e * 0.39894228f; }
-    case kActSilu: { const float s = sigmoid(z); return fabsf(z) == INFINITY ? s : s * (1.f + z * (1.f - s)); }
-    default: return 1.f;
+    default: { const float s = sigmoid(z); return fabsf(z) == INFINITY ? s : s * (1.f + z * (1.f - s)); }      // silu
   }
 }
 // What the forward pass keeps of z for the backward pass.  relu and leakyrelu: one bit (z > 0), a byte per eight columns.  The others:
@@ -1332,14 +1330,12 @@ bool few_rows(uint32_t M, uint32_t N, uint32_t K) { return M <= 512 && (uint64_t
 
 bool dtype16(int d) { return d == SL_BF16 || d == SL_F16; }
 
-template <typename T, int BM_, int BN_, int WM, int WN, int ST, int OCC, int PERCU>
-void nt_tiles(GemmArgs a, bool direct, hipStream_t st) {
+template <typename T, int BM_, int BN_, int WM, int WN, int OCC, int PERCU, bool DIRECT>
+void nt_tiles(GemmArgs a, hipStream_t st) {
   a.tiles_m = (a.M + BM_ - 1) / BM_; a.tiles_n = (a.N + BN_ - 1) / BN_;
   const uint32_t tiles = a.tiles_m * a.tiles_n, most = 256 * PERCU;       // (a multiple of eight: a workgroup stays on its XCD's tiles)
-  const dim3 b(WM * WN * 64);
   // (nothing of the next tile is on its way in the form through registers: a workgroup per tile there)
-  if (direct) hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, ST, OCC, true>), dim3(tiles < most ? tiles : most), b, 0, st, a);
-  else hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, false>), dim3(tiles), b, 0, st, a);
+  hipLaunchKernelGGL((nt_kernel<T, BM_, BN_, WM, WN, 2, OCC, DIRECT>), dim3(DIRECT && tiles > most ? most : tiles), dim3(WM * WN * 64), 0, st, a);
 }
 
 template <typename T, int SIDE>
@@ -1419,9 +1415,11 @@ void nt_launch(GemmArgs a, hipStream_t st) {
     f.g = a;
     few_launch<T, false>(f, direct, st);
   } else if (direct && tiles >= 1024 && a.K >= 512 && a.N >= 256) {
-    nt_tiles<T, 256, 256, 2, 4, 2, 2, 1>(a, direct, st);
+    nt_tiles<T, 256, 256, 2, 4, 2, 1, true>(a, st);
+  } else if (direct) {
+    nt_tiles<T, 128, 128, 2, 2, 2, 2, true>(a, st);
   } else {
-    nt_tiles<T, 128, 128, 2, 2, 2, 2, 2>(a, direct, st);
+    nt_tiles<T, 128, 128, 2, 2, 2, 2, false>(a, st);
   }
 }
 

@@ -7,10 +7,8 @@
 #include <torch/extension.h>
 
 #include <cmath>
-#include <mutex>
 #include <optional>
 #include <string>
-#include <unordered_map>
 
 #include "shadow_hip.h"
 
