@@ -924,7 +924,7 @@ int sl_gat_bwd_map(const uint32_t *d_indptr, const uint32_t *d_indices, const ui
                    const float *d_dnagg_rows, const float *d_t_rows, const uint32_t *d_dn_map, float *d_work, float *d_dz_self,
                    float *d_dz_neigh, float *d_datt, int accumulate_dz_self, float *d_row_amax, void *stream);
 
-/* ---------------------------------------------------------------- node-wise MLP operators (ABI 26)
+/* ---------------------------------------------------------------- node-wise MLP operators (ABI 26; 27: sl_linear16_bwd_scratch_bytes_for)
  * Element types of the operands.  Rows have a pitch (ld*, in elements, at least the row's width); no alignment is required --
  * rows of whole 16-byte words take the fastest path.  Statistics, sums and scores are fp32 whatever the type.  Nothing is allocated,
  * cleared with a memset node or kept between calls: every entry may be captured into a graph. */
@@ -954,9 +954,13 @@ int sl_dropout(int dtype, const void *d_x, int64_t ldx, const void *d_res, int64
 size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N);
 int sl_linear16_fwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, int bias_f32, const void *d_res,
                     int64_t ldr, uint32_t M, uint32_t N, uint32_t K, int act, void *d_y, int64_t ldy, void *d_kept, void *stream);
-/* dx [M, K], dW [N, K], db [N] (each may be NULL; db only together with dW) from dy and d_kept (act != 0).  d_scratch: 16-byte aligned.
- * The rows of dz^T x are cut into slices whose products are added in slice order (no atomics). */
+/* dx [M, K], dW [N, K], db [N] (each may be NULL; db only together with dW) from dy and d_kept (act != 0).  d_scratch: 16-byte aligned,
+ * not NULL, of sl_linear16_bwd_scratch_bytes_for(the call's own operands; want_dx: d_dx given, want_dw: d_dw given) bytes -- or of
+ * sl_linear16_bwd_scratch_bytes, the most that any operands of the shape need (289127 x 256 -> 256: 214 MB, of which a relu's gradients of
+ * rows of whole 16-byte words take 66).  The rows of dz^T x are cut into slices whose products are added in slice order (no atomics). */
 size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K);
+size_t sl_linear16_bwd_scratch_bytes_for(int act, const void *d_x, int64_t ldx, int64_t ldw, const void *d_dy, int64_t lddy, uint32_t M,
+                                         uint32_t N, uint32_t K, int want_dx, int want_dw);
 int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy, const void *d_kept,
                     uint32_t M, uint32_t N, uint32_t K, int act, void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, void *d_db, int db_f32,
                     void *d_scratch, void *stream);

@@ -272,6 +272,7 @@ SIGNATURES = {
                                   _P, C.c_int64, _P, _P]),
     "sl_linear16_kept_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32]),
     "sl_linear16_bwd_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "sl_linear16_bwd_scratch_bytes_for": (C.c_size_t, [C.c_int, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_int]),
     "sl_linear16_bwd": (C.c_int, [C.c_int, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
                                   _P, C.c_int64, _P, C.c_int64, _P, C.c_int, _P, _P]),
     "sl_label_logprobs_scratch_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32]),
@@ -284,7 +285,7 @@ _lib = None
 
 
 MAX_BATCHES_PER_CALL = 16      # SG_MAX_BATCHES_PER_CALL of include/shadow_hip.h
-ABI_VERSION = 26      # sg_abi_version() of the library these signatures describe
+ABI_VERSION = 27      # sg_abi_version() of the library these signatures describe
 
 
 def load():

@@ -1297,18 +1297,49 @@ bool narrow_dw_shape(uint32_t M, uint32_t N, uint32_t K) { return narrow_shape(M
 // dx of so few outputs goes through nt_short_kernel (its wavefronts hold 64 steps of the contraction)
 constexpr uint32_t kShort = 64;
 
+inline uint64_t tiles128(uint32_t M, uint32_t N) { return (uint64_t)((M + 127) / 128) * ((N + 127) / 128); }
+
+// dz^T x in one launch of 32 x 32 tiles: 256 rows of 256 x 256 take 8 us so and 17 in slices of 128 x 128 tiles (dz, product, join),
+// 1024 rows 24 and 18
+bool few_rows(uint32_t M, uint32_t N, uint32_t K) { return M <= 512 && (uint64_t)((N + 31) / 32) * ((K + 31) / 32) <= 1024; }
+
+// Which kernels a backward pass goes through, and what they need in memory.
+struct BwdWay {
+  bool dy_words, dz_words;                   // rows of whole words: dy's, and those of what dx and dW read
+  bool narrow_dx, few_dx, short_dx, narrow_dw, bits_dw, few_dw, tiles_dw;
+  bool need_dz, need_wt;                     // dz and the transposed weight in the scratch
+};
+// small_w: the weight's pitch is below 2^22 elements
+BwdWay way_of(int act, uint32_t M, uint32_t N, uint32_t K, bool dy_words, bool x_words, bool small_w, bool want_dx, bool want_dw) {
+  BwdWay w;
+  w.dy_words = dy_words;
+  // a dy of few columns whose rows are not whole words is first laid out in such rows: loads of unaligned rows, many times over, cost
+  // more (dx and dW of 20011 x 47 -> 500: 43 us so, 35 with the pass; 289127 x 47 -> 256: 152 and 117; 289127 x 172 -> 128: 120 and 133)
+  const bool pad = !act && !dy_words && N <= kShort;
+  w.dz_words = act || pad || dy_words;
+  w.narrow_dx = want_dx && narrow_shape(M, N, K) && w.dz_words;
+  w.few_dx = want_dx && M && !w.narrow_dx && tiles128(M, K) < 64;
+  w.short_dx = want_dx && M && !w.narrow_dx && !w.few_dx && N <= kShort && small_w;
+  w.narrow_dw = want_dw && narrow_dw_shape(M, N, K) && x_words && w.dz_words;
+  w.bits_dw = w.narrow_dw && keeps_bits(act) && dy_words;              // (dz^T x masks dy itself)
+  w.few_dw = want_dw && M && !w.narrow_dw && few_rows(M, N, K);
+  w.tiles_dw = want_dw && !w.narrow_dw && !w.few_dw;
+  // dz in memory, in rows of whole words, unless what reads it forms it itself
+  w.need_dz = M && (act || pad) && ((want_dx && !w.few_dx && !(w.narrow_dx && dy_words)) || (want_dw && !w.bits_dw && !w.few_dw));
+  w.need_wt = want_dx && M && !w.narrow_dx && !w.few_dx && !w.short_dx;
+  return w;
+}
+
 struct BwdPlan {
   uint32_t slices, per;                      // of dz^T x
-  bool narrow;
   uint64_t dz, wt, part, part_b, total;      // byte offsets in the scratch
 };
 
-BwdPlan plan_bwd(uint32_t M, uint32_t N, uint32_t K, bool narrow) {
+BwdPlan plan_bwd(uint32_t M, uint32_t N, uint32_t K, const BwdWay &w) {
   BwdPlan p;
-  p.narrow = narrow;
   const uint64_t tiles = (uint64_t)((N + BN - 1) / BN) * ((K + BM - 1) / BM);
   // row slices of dz^T x: one workgroup per CU, at least four stages each
-  uint32_t s = narrow || tiles == 0 ? 256 : (uint32_t)(256 / tiles);
+  uint32_t s = w.narrow_dw || tiles == 0 ? 256 : (uint32_t)(256 / tiles);
   const uint32_t most = (M + 4 * BK - 1) / (4 * BK);
   s = s < 1 ? 1 : s;
   s = s > most ? most : s;
@@ -1316,17 +1347,13 @@ BwdPlan plan_bwd(uint32_t M, uint32_t N, uint32_t K, bool narrow) {
   p.per = (uint32_t)up((M + s - 1) / s, BK);
   p.slices = M ? (M + p.per - 1) / p.per : 1;
   uint64_t at = 0;
-  p.dz = at; at += up((uint64_t)M * up(N, 8) * 2, 256);
-  p.wt = at; at += up((uint64_t)K * up(N, 8) * 2, 256);
-  p.part = at; at += p.slices > 1 || narrow ? up((uint64_t)p.slices * N * K * 4, 256) : 0;
-  p.part_b = at; at += up((uint64_t)p.slices * N * 4, 256);
+  p.dz = at; at += w.need_dz ? up((uint64_t)M * up(N, 8) * 2, 256) : 0;
+  p.wt = at; at += w.need_wt ? up((uint64_t)K * up(N, 8) * 2, 256) : 0;
+  p.part = at; at += w.narrow_dw || (w.tiles_dw && p.slices > 1) ? up((uint64_t)p.slices * N * K * 4, 256) : 0;
+  p.part_b = at; at += w.narrow_dw || w.tiles_dw ? up((uint64_t)p.slices * N * 4, 256) : 0;
   p.total = at;
   return p;
 }
-
-// dz^T x in one launch of 32 x 32 tiles: 256 rows of 256 x 256 take 8 us so and 17 in slices of 128 x 128 tiles (dz, product, join),
-// 1024 rows 24 and 18
-bool few_rows(uint32_t M, uint32_t N, uint32_t K) { return M <= 512 && (uint64_t)((N + 31) / 32) * ((K + 31) / 32) <= 1024; }
 
 bool dtype16(int d) { return d == SL_BF16 || d == SL_F16; }
 
@@ -1364,8 +1391,6 @@ void tn_narrow_launch(const TnNarrowArgs &n, hipStream_t st) {
     else hipLaunchKernelGGL((tn_narrow_kernel<T, 2, 4, 4, BITS>), g, dim3(512), 0, st, n);
   }
 }
-
-inline uint64_t tiles128(uint32_t M, uint32_t N) { return (uint64_t)((M + 127) / 128) * ((N + 127) / 128); }
 
 template <typename T, bool COLS>
 void few_launch(FewArgs f, bool words, hipStream_t st) {
@@ -1475,9 +1500,19 @@ extern "C" size_t sl_linear16_kept_bytes(int act, uint32_t M, uint32_t N) {
 }
 
 extern "C" size_t sl_linear16_bwd_scratch_bytes(int act, uint32_t M, uint32_t N, uint32_t K) {
-  (void)act;
-  const uint64_t a = plan_bwd(M, N, K, false).total, b = narrow_dw_shape(M, N, K) ? plan_bwd(M, N, K, true).total : 0;
-  return a > b ? a : b;
+  uint64_t most = 0;                         // over every alignment and pitch; what is not asked for only takes away
+  for (int i = 0; i < 8; i++) {
+    const bool dy_words = i & 1, x_words = i & 2, small_w = i & 4;
+    if ((dy_words && N % 8) || (x_words && K % 8)) continue;
+    const uint64_t b = plan_bwd(M, N, K, way_of(act, M, N, K, dy_words, x_words, small_w, true, true)).total;
+    most = b > most ? b : most;
+  }
+  return most;
+}
+
+extern "C" size_t sl_linear16_bwd_scratch_bytes_for(int act, const void *d_x, int64_t ldx, int64_t ldw, const void *d_dy, int64_t lddy, uint32_t M,
+                                                    uint32_t N, uint32_t K, int want_dx, int want_dw) {
+  return plan_bwd(M, N, K, way_of(act, M, N, K, rows_of_words(d_dy, lddy, N, SL_BF16), rows_of_words(d_x, ldx, K, SL_BF16), ldw < (1 << 22), want_dx, want_dw)).total;
 }
 
 extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_dy, int64_t lddy,
@@ -1492,19 +1527,12 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
   if (d_db && !d_dw) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: db comes with dW");
   if (((uint64_t)(K + 31) / 32) * (((uint64_t)N + 31) / 32) > kMaxTiles) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: weight of %u x %u", N, K);
   hipStream_t st = (hipStream_t)stream;
-  const bool dy_words = rows_of_words(d_dy, lddy, N, SL_BF16), x_words = rows_of_words(d_x, ldx, K, SL_BF16), shape = narrow_shape(M, N, K);
-  // a dy of few columns whose rows are not whole words is first laid out in such rows: loads of unaligned rows, many times over, cost
-  // more (dx and dW of 20011 x 47 -> 500: 43 us so, 35 with the pass; 289127 x 47 -> 256: 152 and 117; 289127 x 172 -> 128: 120 and 133)
-  const bool pad = !act && !dy_words && N <= kShort, dz_words = act || pad || dy_words;
-  const bool narrow_dx = d_dx && shape && dz_words, narrow_dw = want_w && narrow_dw_shape(M, N, K) && x_words && dz_words;
-  const bool bits_dw = narrow_dw && keeps_bits(act) && dy_words;       // (dz^T x masks dy itself)
-  const bool few_dx = d_dx && M && !narrow_dx && tiles128(M, K) < 64, few_dw = want_w && M && !narrow_dw && few_rows(M, N, K),
-             short_dx = d_dx && M && !narrow_dx && !few_dx && N <= kShort && ldw < (1 << 22);
-  const BwdPlan p = plan_bwd(M, N, K, narrow_dw);
-  if (d_dx && !narrow_dx && !short_dx && takes_few(M, K, N, lddy, 0) && !few_fits(M, K)) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: too many tiles");
+  const bool x_words = rows_of_words(d_x, ldx, K, SL_BF16);
+  const BwdWay w = way_of(act, M, N, K, rows_of_words(d_dy, lddy, N, SL_BF16), x_words, ldw < (1 << 22), d_dx != nullptr, want_w);
+  const BwdPlan p = plan_bwd(M, N, K, w);
+  const bool dy_words = w.dy_words, need_dz = w.need_dz, narrow_dx = w.narrow_dx, narrow_dw = w.narrow_dw;
+  if (d_dx && !narrow_dx && !w.short_dx && takes_few(M, K, N, lddy, 0) && !few_fits(M, K)) return set_error(SG_ERR_INVALID, "sl_linear16_bwd: too many tiles");
   char *ws = static_cast<char *>(d_scratch);
-  // dz in memory, in rows of whole words, unless what reads it forms it itself
-  const bool need_dz = M && (act || pad) && ((d_dx && !few_dx && !(narrow_dx && dy_words)) || (want_w && !bits_dw && !few_dw));
   const int64_t ldp = (int64_t)up(N, 8);
   const void *dz = need_dz ? ws + p.dz : d_dy;
   const int64_t lddz = need_dz ? ldp : lddy;
@@ -1527,20 +1555,20 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
                     else if (keeps_bits(act)) narrow_launch<T, 3>(n, st);
                     else narrow_launch<T, 2>(n, st));
     SHD_HIP(hipGetLastError());
-  } else if (few_dx) {
+  } else if (w.few_dx) {
     FewArgs f = {};
     f.g.A = dz; f.g.lda = lddz; f.g.B = d_w; f.g.ldb = ldw; f.g.M = M; f.g.N = K; f.g.K = N; f.g.C = d_dx; f.g.ldc = lddx;
     f.kept = static_cast<const char *>(d_kept); f.kept_act = need_dz ? 0 : act;
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
     SHD_DISPATCH_16(dtype, few_launch<T, true>(f, rows_of_words(dz, lddz, N, SL_BF16), st));
     SHD_HIP(hipGetLastError());
-  } else if (short_dx) {
+  } else if (w.short_dx) {
     GemmArgs a = {};
     a.A = dz; a.lda = lddz; a.B = d_w; a.ldb = ldw; a.M = M; a.N = K; a.K = N; a.C = d_dx; a.ldc = lddx;
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dx_N%u_K%u", N, K);
     SHD_DISPATCH_16(dtype, short_launch<T>(a, st));
     SHD_HIP(hipGetLastError());
-  } else if (d_dx && M) {
+  } else if (w.need_wt) {
     GemmArgs a = {};
     a.A = dz; a.lda = lddz; a.B = ws + p.wt; a.ldb = ldp; a.M = M; a.N = K; a.C = d_dx; a.ldc = lddx;
     a.K = need_dz ? (uint32_t)ldp : N;       // (pad columns are zero on both sides: whole words)
@@ -1550,7 +1578,7 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
                     nt_launch<T>(a, st));
     SHD_HIP(hipGetLastError());
   }
-  if (few_dw) {
+  if (w.few_dw) {
     TnFewArgs f = {};
     TnArgs &a = f.t;
     a.A = dz; a.lda = lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + 31) / 32; a.tiles_k = (K + 31) / 32; a.C = d_dw; a.ldc = lddw;
@@ -1561,15 +1589,15 @@ extern "C" int sl_linear16_bwd(int dtype, const void *d_x, int64_t ldx, const vo
   } else if (want_w) {
     TnNarrowArgs n = {};
     TnArgs &a = n.t;
-    a.A = bits_dw ? d_dy : dz; a.lda = bits_dw ? lddy : lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + BN - 1) / BN;
+    a.A = w.bits_dw ? d_dy : dz; a.lda = w.bits_dw ? lddy : lddz; a.B = d_x; a.ldb = ldx; a.M = M; a.N = N; a.K = K; a.tiles_n = (N + BN - 1) / BN;
     a.tiles_k = (K + BM - 1) / BM; a.slices = p.slices; a.per = p.per; a.C = d_dw; a.ldc = lddw;
-    a.part = p.slices > 1 || narrow_dw ? reinterpret_cast<float *>(ws + p.part) : nullptr;
+    a.part = narrow_dw || p.slices > 1 ? reinterpret_cast<float *>(ws + p.part) : nullptr;
     a.part_b = d_db ? reinterpret_cast<float *>(ws + p.part_b) : nullptr;
     n.kept = static_cast<const char *>(d_kept); n.kept_act = act;
     const uint64_t joined = (a.part ? (uint64_t)N * K : 0) + (d_db ? N : 0);
     SHD_PROF_FMT(bytes_dx, 2.0 * M * N * K, st, "linear16_dw_N%u_K%u", N, K);
-    SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, dz_words, x_words, st);
-                    else if (bits_dw) tn_narrow_launch<T, true>(n, st);
+    SHD_DISPATCH_16(dtype, if (!narrow_dw) tn_launch<T>(a, w.dz_words, x_words, st);
+                    else if (w.bits_dw) tn_narrow_launch<T, true>(n, st);
                     else tn_narrow_launch<T, false>(n, st);
                     if (joined) hipLaunchKernelGGL((tn_join_kernel<T>), dim3((uint32_t)((joined + 63) / 64)), dim3(256), 0, st, a.part, a.part_b, p.slices, N, K,
                                                    (T *)d_dw, lddw, d_db, db_f32));

@@ -296,7 +296,7 @@ struct LinearAct : public Function<LinearAct> {
       Tensor dW;
       if (need_w || need_b) dW = like(x, {(int64_t)N, (int64_t)K});
       if (need_b) out[2] = like(x, {(int64_t)N}, (at::ScalarType)bias);
-      const Tensor ws = like(x, {(int64_t)sl_linear16_bwd_scratch_bytes(act, M, N, K) + 16}, at::kByte);
+      const Tensor ws = like(x, {(int64_t)sl_linear16_bwd_scratch_bytes_for(act, r.p, r.ld, w.ld, d.p, d.ld, M, N, K, need_x, need_w || need_b) + 16}, at::kByte);
       const On on(x);
       check(sl_linear16_bwd(dtype_of(x), r.p, r.ld, w.p, w.ld, d.p, d.ld, ptr(kept), M, N, K, act, ptr(out[0]), K, ptr(dW), K, ptr(out[2]),
                             bias == (int64_t)at::kFloat, ws.data_ptr(), on.stream));

@@ -149,3 +149,29 @@ def test_sizes_of_scratch():
     assert lib.sl_linear16_kept_bytes(0, 10, 64) == 0 and lib.sl_linear16_kept_bytes(1, 10, 129) == 320 and lib.sl_linear16_kept_bytes(5, 10, 129) == 10 * 136 * 2
     # the largest weight of the documented range (2^34 tiles): a size, not a division by their number in 32 bits
     assert lib.sl_linear16_bwd_scratch_bytes(0, 1000, 1 << 24, 1 << 24) > 1 << 48
+
+
+def test_scratch_of_a_backward_call():
+    """The scratch holds what a call goes through memory with: dz where a kernel reads it, the transposed weight where it is read, partial
+    products where rows are cut into slices; the size by the shape alone covers every alignment, pitch and set of gradients."""
+    lib = _lib.load()
+
+    def size(act, M, N, K, x=P, ldx=None, ldw=None, dy=P, lddy=None, dx=1, dw=1):
+        return lib.sl_linear16_bwd_scratch_bytes_for(act, x, ldx or K, ldw or K, dy, lddy or N, M, N, K, dx, dw)
+
+    M, dz, part = 289127, 289127 * 256 * 2, 251 * 256 * 256 * 4               # (slices of 18 stages of 64 rows: 251)
+    assert size(0, M, 256, 256) < part + (1 << 20)                              # an identity reads dy as it is
+    assert size(1, M, 256, 256) < part + (1 << 20)                              # relu: both products mask dy themselves
+    assert dz + part < size(5, M, 256, 256) < dz + part + (1 << 20)             # gelu: dx forms dz, dW reads it
+    assert dz + part < size(1, M, 256, 256, dy=P + 2) < dz + part + (1 << 20)   # rows of dy that are not whole words
+    assert size(5, M, 256, 256, dw=0) == 0                                      # dx alone: no dz in memory
+    assert size(1, 256, 256, 256) == 0                                          # few rows: nothing
+    assert size(0, 32768, 4096, 1024, dw=0) == 4096 * 1024 * 2                  # a wide dx: the transposed weight
+    assert size(2, 32768, 4096, 1024) == 4096 * (1024 + 32768) * 2 + 4096 * 4
+    for act in (0, 1, 5):
+        for M in (0, 1, 300, 513, 5000, 20011, 98304):
+            for N in (1, 40, 47, 64, 72, 256, 1000, 1001):
+                for K in (1, 8, 100, 256, 1024, 1001):
+                    most = lib.sl_linear16_bwd_scratch_bytes(act, M, N, K)
+                    for x, dy, ldw, dx, dw in ((P, P, K, 1, 1), (P + 2, P, K, 1, 1), (P, P + 2, K, 1, 1), (P + 2, P + 2, 1 << 22, 1, 1), (P, P, K, 1, 0), (P, P + 2, K, 0, 1)):
+                        assert size(act, M, N, K, x=x, dy=dy, ldw=ldw, dx=dx, dw=dw) <= most

@@ -685,6 +685,36 @@ def test_linear16_writes_its_own_elements_only(M, N, K, act):
         assert (t[:, width:] == 77).all() and (t[n:] == 77).all() and (t[:n, :width] != 77).any(1).all()
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("wants", ["both", "dx", "dW"])
+@pytest.mark.parametrize("M,N,K,act", [(98309, 256, 256, 1), (98309, 136, 72, 5), (98309, 72, 136, 0), (98309, 47, 256, 0), (16411, 128, 72, 4), (16393, 40, 16, 0), (1111, 1100, 264, 2),
+                                       (1111, 1100, 264, 0), (530, 300, 100, 1), (512, 304, 104, 5), (9000, 40, 1024, 0), (9000, 72, 1024, 0)])
+def test_linear16_backward_stays_in_the_scratch_of_its_call(M, N, K, act, wants, shift):
+    """sl_linear16_bwd with exactly the scratch stated for its operands: what lies behind stays as it was, the gradients are those of a
+    call with the shape's largest scratch."""
+    from shadow_gnn_amd import _lib
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    g = _gen(65)
+    x, W, dy = _randn(g, M, K, dtype=BF16), _randn(g, N, K, dtype=BF16, scale=K ** -0.5), _randn(g, M * N + 8, dtype=BF16)[shift:][:M * N].view(M, N)
+    y, kept = torch.empty_like(dy), torch.empty(lib.sl_linear16_kept_bytes(act, M, N) + 16, dtype=torch.uint8, device=DEV)
+    assert lib.sl_linear16_fwd(1, x.data_ptr(), K, W.data_ptr(), K, None, 0, None, 0, M, N, K, act, y.data_ptr(), N, kept.data_ptr() if act else None, st) == 0
+    most = lib.sl_linear16_bwd_scratch_bytes(act, M, N, K)
+    exact = lib.sl_linear16_bwd_scratch_bytes_for(act, x.data_ptr(), K, K, dy.data_ptr(), N, M, N, K, wants != "dW", wants != "dx")
+    assert exact <= most
+    got = []
+    for size in (exact, most):
+        ws = torch.full((size + 4096,), 0x5A, dtype=torch.uint8, device=DEV)
+        dx, dw, db = torch.zeros(M, K, dtype=BF16, device=DEV), torch.zeros(N, K, dtype=BF16, device=DEV), torch.zeros(N, device=DEV)
+        assert lib.sl_linear16_bwd(1, x.data_ptr(), K, W.data_ptr(), K, dy.data_ptr(), N, kept.data_ptr() if act else None, M, N, K, act,
+                                   dx.data_ptr() if wants != "dW" else None, K, dw.data_ptr() if wants != "dx" else None, K,
+                                   db.data_ptr() if wants != "dx" else None, 1, ws.data_ptr(), st) == 0
+        torch.cuda.synchronize()
+        assert (ws[size:] == 0x5A).all()
+        got.append((dx, dw, db))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert got[0][0].any() == (wants != "dW") and got[0][1].any() == (wants != "dx")
+
+
 def test_gradients_are_differentiable_once():
     """create_graph gives the same gradients; a second backward pass through them is an error, not zeros."""
     from shadow_gnn_amd import ops_mlp
