@@ -14,9 +14,10 @@
 //
 // Two forms of the forward pass (forward_in_registers() has the rule): rows of up to 1024 classes stay in the registers of 4 to 64
 // lanes; longer ones are streamed by a workgroup each -- by several, joined by a second kernel, where there are few rows.
-// 289127 x 172 fp32: forward 32 us without alternatives (6.2 TB/s), 68 with five (each is a round of compares over the row's registers);
-// backward 70 us (5.7 TB/s).  2048 x 131072 bf16: forward 99 us (5.4 TB/s; eleven operations per element run beside the
-// loads), backward 177 us (6.1 TB/s).  1 x 131072 fp16 with ten alternatives: 8.4 + 7.0 us, the latency of two launches and of the lists.
+// 289127 x 172 fp32: forward 32 to 39 us without alternatives (6.2 to 5.1 TB/s), 68 to 72 with five (each is a round of compares over the
+// row's registers); backward 70 us (5.7 TB/s).  289127 x 47 fp32 (one element per load): 17 and 26 us.  2048 x 131072 bf16: forward 99 us
+// (5.4 TB/s; eleven operations per element run beside the loads), 190 with ten alternatives (their lists leave no registers for loads ahead);
+// backward 177 us (6.1 TB/s).  1 x 131072 fp16 with ten alternatives: 8.4 + 7.0 us, the latency of two launches and of the lists.
 #include "elem.h"
 
 using namespace shadow;
@@ -545,8 +546,9 @@ __device__ __forceinline__ float grad_of(const RowGrad &g, float x) {
   return -p * __builtin_fmaf(g.h, __builtin_fmaf(kLn2, u, g.H), g.neg);
 }
 
-// V elements per step; LPR lanes (a power of two) walk a row, workgroups walk (row, part) pairs.  The one-hot terms of the
-// alternatives are put in by a second look at those elements (k of them) after the row's part is written.
+// V elements per step; `lanes` lanes (a power of two) walk a row, workgroups walk (row, part) pairs.  The one-hot terms of the
+// alternatives go in before the one rounding: every word is held against the row's k indices, which are read again for each (289127 x 172
+// fp32: 72 us without their gradient, 192 with that of five).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwdArgs a, uint32_t lanes, uint32_t parts, uint32_t per) {
   const uint32_t nch = a.C / V, sub = threadIdx.x & (lanes - 1), G = 256 / lanes;
@@ -585,7 +587,9 @@ __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwdArgs a, uint32_t lanes
 // the rule: a row that 64 lanes hold at 16 elements each
 bool forward_in_registers(uint32_t C) { return C <= 1024; }
 
-// parts of a streamed row: enough workgroups for two per CU, at least one trip's words each
+// parts of a streamed row: enough workgroups for two per CU, at least one trip's words each.  (64 rows of 131072 bf16 with ten
+// alternatives take 31 us with one workgroup per CU, 25 so and 22 with four; without alternatives 9.4, 9.6 and 9.8; 256 rows 14.5, 17 and
+// 18, 512 rows 28, 28 and 34.)
 uint32_t splits_of(uint32_t n, uint32_t C, int dtype) {
   const uint32_t trip = kStreamThreads * kStreamWords * (16u / elem_bytes(dtype));
   const uint32_t most = (C + trip - 1) / trip, want = (512u + n - 1) / n;

@@ -9,7 +9,9 @@
 // The weight gradient: every lane keeps its columns' running sums over the rows its workgroup walks (registers, no atomics), a
 // workgroup leaves one row of partial sums, and a second kernel adds those in a fixed order -- the same bits every time.
 // 289127 x 256 bf16: forward 61 us (4.8 TB/s), backward 87 us (5.1 TB/s) + 4.8 for the weight gradient, where a large copy runs at 5.2;
-// 16385 x 800 fp16 12.5 and 18 + 4; 1024 x 256 fp32 forward 2.9.
+// 16385 x 800 fp16 12.5 and 18 + 4; 1024 x 256 fp32 forward 2.9; 289127 x 256 fp32 105 and 178 + 5.  Rows that are not whole 16-byte words
+// go one element per load: 50021 x 602 fp32 48 and 71 + 5 (5.0 TB/s: a wavefront still reads whole lines), 20011 x 500 bf16 21 and 24 + 4
+// (1.9 and 2.5 TB/s: half lines).
 #include "elem.h"
 
 using namespace shadow;
@@ -257,7 +259,8 @@ int lanes_of(uint32_t F) {
 }
 
 // up to this many trips one workgroup takes all rows and writes the weight gradient itself: a launch (some 4 us of the host's time)
-// less than it costs
+// less than it costs.  On the GPU one workgroup and several with the second launch take 5.5 and 6.6 us for 32 rows of 256 bf16 (two
+// trips), 7.1 and 6.7 for 64 (four), 10 and 6.7 for 128; 20 and 22 for 2 rows of 16384, 24 and 22 for 4.
 constexpr uint32_t kAlone = 4;
 
 uint32_t bwd_blocks(uint32_t n, uint32_t F) {

@@ -10,8 +10,10 @@
 // crossed to the CU twice, 338 instead of 314 us at 32768 x 1024 x 4096 -- and multiplied on 32x32x16 products formed as W x^T: a lane then
 // holds four neighbouring output COLUMNS of a row.
 // 32768 x 1024 x 4096 fp16 gelu: 352 us, 215 to 226 of them the main loop (1.2 PFLOP/s; the products alone 166, and LDS is busy as long)
-// and the rest an epilogue that does not overlap with it (two workgroups per CU of 128 x 256 tiles and half stages, whose would: 412).  289127 x 256 x 256 bf16 relu with residual (bound by memory): forward 105 us, dx 95, dW 83 + 12.
-// 256 x 256 x 256: 4.8 us.
+// and the rest an epilogue that does not overlap with it (two workgroups per CU of 128 x 256 tiles and half stages, whose would: 412) and
+// the wait for its stores: they count in vmcnt, and the first stage after them waits for vmcnt(0).
+// 289127 x 256 x 256 bf16 relu with residual: forward 105 us (bound by memory), dx 95 (59 by memory; see narrow_kernel), dW 83 + 12.
+// 256 x 256 x 256: 4.8 us.  20011 x 1024 -> 1024 bf16 gelu: forward 80, dx 68 to 95, dz 26, dW 92 + 9 (products: 29 each).
 // Operands whose rows are whole 16-byte words go to LDS directly (global_load_lds, no registers); any other pitch or width is loaded
 // into registers (unaligned 16-byte loads, the last word of a row element by element) and written from there.
 #include "elem.h"
@@ -34,8 +36,9 @@ __device__ __forceinline__ f32x16 mma(Frag<f16_t>::v8 a, Frag<f16_t>::v8 b, f32x
 
 constexpr int kActGelu = 5, kActSilu = 6, kActs = 7;
 
-// Phi(z) and the density's exp(-z^2 / 2): erfc by Abramowitz & Stegun 7.1.26 (absolute error below 1.5e-7, a hundredth of a bf16 or
-// fp16 step of the result), whose exponential is the density's
+// Phi(z) and the density's exp(-z^2 / 2): erfc by Abramowitz & Stegun 7.1.26, whose exponential is the density's.  Its error is an
+// absolute one, below 1.5e-7.  Against the result that is next to nothing where |z Phi(z)| is of z's size, but the negative tail is small
+// itself: gelu is off by a third of an fp16 step at z = -3.5, half of one at -4, and by 0.3, 0.7 and 1 bf16 step at -5, -6 and -7.
 __device__ __forceinline__ void normal_cdf(float z, float &cdf, float &ex) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.3275911f * 0.70710678f, 1.f));
   ex = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504f));
@@ -75,14 +78,17 @@ __device__ __forceinline__ float slope16(int act, float z) {
   }
 }
 // What the forward pass keeps of z for the backward pass.  relu and leakyrelu: one bit (z > 0), a byte per eight columns.  The others:
-// z in fp16 whatever the operands' type -- eleven bits keep act'(z) well inside a bf16 step, and where fp16's range ends every slope
-// has reached its limit.
+// z in fp16 whatever the operands' type (half the bytes of fp32; bf16 would keep three bits less).  Rounding z moves act'(z) by at most
+// 0.3 x 2^-11 (gelu, silu), 0.36 (elu) or 0.63 (tanh): less than an fp16 step of a slope near 1.  Where the slope is small itself that
+// is more of it: 0.4 to 0.8 % of tanh's beyond |z| = 4 (below 1.4e-3), 0.4 % of elu's below -8, 1.6 % and more of gelu's below -4.
+// Where fp16's range ends every slope has reached its limit.
 __host__ __device__ constexpr bool keeps_bits(int act) { return act == 1 || act == 4; }
 __host__ __device__ constexpr uint64_t up(uint64_t v, uint64_t m) { return (v + m - 1) / m * m; }
 // bytes of a kept row: whole 16-byte words
 __host__ __device__ constexpr uint64_t kept_pitch(int act, uint32_t N) { return keeps_bits(act) ? up((N + 7) / 8, 16) : up(N, 8) * 2; }
 
-// eight elements of dz = dy act'(z), rounded to the operands' type (the products need 16-bit operands; for relu nothing is lost).
+// eight elements of dz = dy act'(z), rounded to the operands' type (the products need 16-bit operands; for relu nothing is lost).  db sums
+// the same rounded dz on the same products: a sum of its own in fp32 would be another pass over dz.
 // z: the word of kept values, or the byte of kept bits in z.x.  A dy of zero is a dz of zero.
 template <typename T>
 __device__ __forceinline__ uint4 dz_word(int act, const uint4 &dy, const uint4 &z) {
@@ -718,6 +724,11 @@ __global__ void __launch_bounds__(256, 4) nt_short_kernel(GemmArgs a, uint32_t g
 // wavefront's own loads and stores and in order: apart from each other, the senders keep RS - 1 tiles on their way and the multiplying
 // wavefronts never wait for their stores (with the residual loaded by them the forward pass took 140, dx 150 us at 289127 x 256 x 256).
 // One barrier per tile: the tile is whole, and the one before it has been read.
+// SIDE 2 and 3 await a tile one turn earlier, so that it can become dz; there RS - 2 tiles are under way at a wait, which counts as the
+// ring's end: everything sent has to arrive, and one tile is on its way beside the products.  dx of 289127 x 256 x 256 takes 95 us of a
+// relu or leakyrelu so (59 by memory) and 300 to 370 of gelu, silu, elu and tanh, whose form in addition spills (176 bytes a lane): dz written
+// by dz_kernel first and dx through SIDE 0 would take 170 to 177 there, 25 instead of 38 us at 20011 x 256 x 256, 78 instead of 142 at
+// 289127 x 128 x 128, with the same bits.
 //   SIDE 1: the residual's rows.
 //   SIDE 2, 3 (dx = dz W; A is dy): kept fp16 values / kept bits.  The tile becomes dz = dy act'(z) in place, each wavefront a share
 //   of it, while the tile before it is multiplied, and is stored for dz^T x if asked for.
@@ -1368,7 +1379,7 @@ void nt_tiles(GemmArgs a, hipStream_t st) {
 template <typename T, int SIDE>
 void narrow_launch(const NarrowArgs &n, hipStream_t st) {
   const uint32_t tiles = (n.g.M + 31) / 32;
-  // (places of the ring by what LDS holds: 96 to 112 KB on their way on a CU)
+  // (places of the ring by what LDS holds: 96 to 112 KB on their way on a CU in SIDE 0 and 1)
 #define SHD_NARROW(NWC, KS, RS, PERCU)                                                                                                  \
   hipLaunchKernelGGL((narrow_kernel<T, NWC, KS, RS, SIDE>), dim3(tiles < 256 * PERCU ? tiles : 256 * PERCU), dim3((NWC + 4) * 64), 0, st, n)
   if (n.g.N <= 128) {
@@ -1415,13 +1426,19 @@ void short_launch(const GemmArgs &a, hipStream_t st) {
 bool few_fits(uint32_t M, uint32_t N) { return (((uint64_t)M + 31) / 32) * (((uint64_t)N + 31) / 32) < 1u << 23; }
 // x W^T in 32 x 32 tiles: fewer than 64 tiles of 128 (1024 x 1024 x 1024, 64 tiles, takes 17.6 us in 32 x 32 tiles and 18.0 in 128 x 128
 // ones, twice the rows 32 and 18.5, 1024 x 256 x 256 4.5 and 9.6, one row of 4096 x 4096 11 and 47), fewer than 128 where half of each were
-// empty (8192 x 1024 -> 40 9.1 and 17.6, 16000 x 500 -> 48 9.4 and 12.8, but 16000 x 2000 -> 64 37 and 32), any number where three quarters
+// empty (8192 x 1024 -> 40 9.1 and 17.6, 16000 x 500 -> 48 9.4 to 11.3 and 12.8 to 14.2, but 16000 x 2000 -> 64 37 and 32; above, the
+// times cross at about 150 tiles: 16512 x 500 -> 48 12.3 and 13.8, 20011 x 500 -> 47 15.0 and 14.7, 30000 19.6 and 15.4, 50000 30 and 20,
+// 20011 x 1000 -> 47 24 and 21, 20011 x 256 -> 47 7.5 and 7.6), any number where three quarters
 // were (30000 x 500 -> 16 8.9 and 14.8, 100000 x 600 -> 8 27 and 38, but 60000 x 1000 -> 32 39 and 31); and what the tile kernel does not
 // hold: its offsets (256 rows of a pitch below 2^22 elements stay below 2^31 bytes) and contractions of less than eight, both rare
 bool takes_few(uint32_t M, uint32_t N, uint32_t K, int64_t lda, int64_t ldb) {
   return tiles128(M, N) < (N <= 64 && K <= 1024 ? 128u : 64u) || (N <= 32 && K <= 640 && few_fits(M, N)) || lda >= (1 << 22) || ldb >= (1 << 22) || K < 8;
 }
 
+// 256 x 256 tiles: from 1024 tiles of 128 on (32768 x 1024 -> 1024 82 us in 256 x 256 tiles and 103 in 128 x 128 ones, 8192 x 1024 -> 2048
+// 41 and 48, 65536 x 512 -> 256 33 and 39, 4096^3 117 and 143; half as many tiles leave CUs idle: 8192 x 1024 -> 1024 35 and 25, 4096 x 4096
+// -> 2048 95 and 72), unless half of each were empty (131072 x 512 -> 128 56 and 47), and of contractions of 512 and more.  (Shorter ones are
+// faster so too -- 65536 x 256 -> 1024 76 and 96, 32768 x 256 -> 1024 37 and 42, 65536 x 384 -> 512 49 and 63 -- and still go to 128 x 128.)
 template <typename T>
 void nt_launch(GemmArgs a, hipStream_t st) {
   const bool direct = rows_of_words(a.A, a.lda, a.K, SL_BF16) && rows_of_words(a.B, a.ldb, a.K, SL_BF16);

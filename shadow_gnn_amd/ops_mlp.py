@@ -41,7 +41,8 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor, None] = No
     """``residual + mask * x / (1 - p)`` for ``0 <= p < 1``, in x's type (one rounding).  The mask is the rule of the fused epilogues
     (``ops.dropout_keep_mask(rows, width, p, seed)``, rows counted over the leading dimensions) and is never stored: the backward pass
     forms it again.  ``seed``: an int; an int64 tensor of one element on x's device, read when the kernel runs (a replayed graph takes
-    the value it holds then; do not change it between a forward pass and its backward pass); None draws ``ops.new_dropout_seed()``.
+    the value it holds then; do not change it between a forward pass and its backward pass); None draws ``ops.new_dropout_seed()`` (a
+    graph captured with an int or None keeps that seed: every replay has the same mask).
     A dropped element is 0 even where x is infinite or NaN."""
     if seed is None:
         seed = new_dropout_seed()
@@ -59,8 +60,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     bias ``[N]`` in that type or fp32; products and the epilogue in fp32, one rounding at the end.  ``act``: a key of
     ``LINEAR_ACT_CODE``.  fp32 operands go through ``ops.linear`` / ``ops.linear_act_norm``.
 
+    A NaN pre-activation stays NaN through every activation but relu, where it is 0 and passes no gradient (the rule of the layers' own
+    relu).
+
     For the backward pass one bit of every pre-activation is kept (relu, leakyrelu) or its fp16 value (the others), and
-    ``dz = dy act'(z)`` is rounded to the operands' type (the matrix cores take 16-bit operands); an identity keeps and rounds nothing."""
+    ``dz = dy act'(z)`` is rounded to the operands' type (the matrix cores take 16-bit operands) before dx, dW and db are formed of it:
+    gradients through elu, tanh, gelu and silu are good to about two half steps of the operands' type instead of one.  An identity keeps
+    and rounds nothing."""
     code = LINEAR_ACT_CODE.get(act)
     if code is None:
         raise NotImplementedError(f"linear_act: activation {act!r} is not provided ({sorted(LINEAR_ACT_CODE)})")
@@ -81,5 +87,6 @@ def label_logprobs(logits: torch.Tensor, label: torch.Tensor, topk: int = 0) -> 
     differentiable in the logits, without an ``[..., C]`` intermediate.
 
     A negative label stands for none: its log probability is 0 and passes no gradient; a label >= C gives NaN.  A logit of -inf has
-    probability 0; a row without a finite logit answers -inf, entropy 0 and gradient 0; +inf or NaN makes its row NaN."""
+    probability 0; a row without a finite logit answers -inf, entropy 0 and gradient 0; +inf or NaN makes its row NaN.  At most 67108856
+    rows (2^24 workgroups' worth where rows are longer than 1024)."""
     return LabelLogprobs(*(_native or _host()).label_logprobs(logits, label, topk))

@@ -421,6 +421,23 @@ def test_linear_act_special_values_stay_in_their_rows():
         _assert_within(gx, want.expand(2, 8), 0.0, act)
 
 
+@pytest.mark.parametrize("M,N,K", [(40, 24, 40), (9000, 24, 40), (9000, 600, 40)])
+def test_linear_act_nan_pre_activations(M, N, K):
+    """A NaN stays NaN through every activation but relu, whose rule makes it 0 and passes no gradient."""
+    from shadow_gnn_amd import ops_mlp
+    g = _gen(36)
+    x, W = _randn(g, M, K, dtype=BF16), _randn(g, N, K, dtype=BF16, scale=0.1)
+    x[M // 2, 3] = float("nan")
+    for act in ("I", "relu", "elu", "tanh", "leakyrelu", "gelu", "silu"):
+        leaf = x.clone().requires_grad_(True)
+        y = ops_mlp.linear_act(leaf, W, act=act)
+        assert y.isnan().any(1).nonzero().tolist() == ([] if act == "relu" else [[M // 2]]), act
+        assert y[M // 2].isnan().all() if act != "relu" else not y[M // 2].any(), act
+        dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        if act == "relu":
+            assert not dx[M // 2].any() and not dx.isnan().any()
+
+
 def test_linear_act_reproducible_and_differences():
     from shadow_gnn_amd import ops_mlp
     g = _gen(35)
