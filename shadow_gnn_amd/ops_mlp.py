@@ -88,5 +88,5 @@ def label_logprobs(logits: torch.Tensor, label: torch.Tensor, topk: int = 0) -> 
 
     A negative label stands for none: its log probability is 0 and passes no gradient; a label >= C gives NaN.  A logit of -inf has
     probability 0; a row without a finite logit answers -inf, entropy 0 and gradient 0; +inf or NaN makes its row NaN.  At most 67108856
-    rows (2^24 workgroups' worth where rows are longer than 1024)."""
+    rows, 16777215 of more than 1024 logits (a workgroup each)."""
     return LabelLogprobs(*(_native or _host()).label_logprobs(logits, label, topk))
